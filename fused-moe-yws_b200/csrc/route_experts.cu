@@ -1,0 +1,420 @@
+// route_experts.cu -- expert routing for any scoring rule, and its gradient.
+//
+//   s   = softmax(x) | sigmoid(x)             over the experts a token may use (x > -inf)
+//   c   = s + bias; without a bias the order of c is the order of x
+//   keep topk_group of n_group groups by the sum of their two largest c (or the largest),
+//   pick top_k of the kept groups' experts by c; ties go to the lower index
+//   w_k = scale * s_k, or renormalised: softmax over the picked experts; for the sigmoid
+//         scale * s_k / (sum_k s_k + 1e-20)
+//
+// The order is decided as exact arithmetic decides it: two scores that differ by less than
+// single precision resolves still have an order, and a different pick changes the token's
+// output. Every selection here runs in 64 bits.
+//
+// One warp routes one token; lane l holds experts l * EPL .. l * EPL + EPL - 1.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <string>
+
+#include "fmoe.h"
+#include "fmoe_common.cuh"
+#include "fmoe_kernels.cuh"
+
+namespace fmoe {
+namespace {
+
+constexpr int kRouterWarps = 8;
+constexpr int kRouterMaxExperts = 1024;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouterArgs {
+  const void* logits;
+  int64_t stride;  // elements between rows of logits
+  const void* bias;  // or null
+  bool bias_bf16;
+  int64_t T;
+  int E, K, n_group, topk_group;
+  bool softmax, group_max, renorm;
+  float scale;
+  int* idx;          // [T, K]
+  float* w;          // [T, K]
+  // backward
+  const float* grad_w;  // [T, K]
+  void* grad_logits;    // [T, E], the type of the logits
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// The lane's logits; experts past E and unusable ones (NaN) become -inf.
+template <int EPL, typename In>
+__device__ __forceinline__ void load_logits(const RouterArgs& a, int64_t t, int lane,
+                                            float (&x)[EPL]) {
+  const In* row = static_cast<const In*>(a.logits) + t * a.stride;
+  const int e0 = lane * EPL;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const float v = e0 + j < a.E ? to_float(row[e0 + j]) : neg_inf();
+    x[j] = v > neg_inf() ? v : neg_inf();
+  }
+}
+
+__device__ __forceinline__ float load_bias(const RouterArgs& a, int e) {
+  return a.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[e])
+                     : static_cast<const float*>(a.bias)[e];
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// exp(x - top) with the top itself at exactly 1, also where it is +inf (which then shares
+// the whole mass with the other infinities, the limit of the softmax).
+__device__ __forceinline__ double exp_below(float x, float top) {
+  return x == top ? 1.0 : exp((double)x - (double)top);
+}
+__device__ __forceinline__ float exp_below_f(float x, float top) {
+  return x == top ? 1.0f : expf(x - top);
+}
+
+// Picks the token's experts: lane k returns the k-th one, or -1.
+template <int EPL>
+__device__ __forceinline__ int select_experts(const RouterArgs& a, const float (&x)[EPL],
+                                              int lane) {
+  const int e0 = lane * EPL;
+  double worth[EPL], c[EPL];
+  if (a.softmax) {
+    float top = neg_inf();
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
+    top = warp_max(top);
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      worth[j] = x[j] > neg_inf() ? exp_below(x[j], top) : 0.0;
+      sum += worth[j];
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) worth[j] = sum > 0.0 ? worth[j] / sum : 0.0;
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) worth[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+  }
+  uint32_t live = 0;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    if (a.bias && e0 + j < a.E) worth[j] += (double)load_bias(a, e0 + j);
+    c[j] = a.bias ? worth[j] : (double)x[j];
+    if (x[j] > neg_inf() && c[j] > (double)neg_inf()) live |= 1u << j;
+  }
+  if (a.n_group > 1) {
+    const int G = a.E / a.n_group;
+    double mine = (double)neg_inf();  // lane g: the score of group g
+    for (int g = 0; g < a.n_group; ++g) {
+      double m1 = (double)neg_inf(), m2 = (double)neg_inf();
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        const int e = e0 + j;
+        if (((live >> j) & 1u) && e >= g * G && e < g * G + G) {
+          const double v = a.group_max ? c[j] : worth[j];
+          m2 = fmax(m2, fmin(m1, v));
+          m1 = fmax(m1, v);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        const double p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
+        m2 = fmax(fmin(m1, p1), fmax(m2, p2));
+        m1 = fmax(m1, p1);
+      }
+      if (lane == g) mine = a.group_max ? m1 : m1 + m2;
+    }
+    int rank = 0;
+    for (int h = 0; h < a.n_group; ++h) {
+      const double v = __shfl_sync(kAll, mine, h);
+      rank += v > mine || (v == mine && h < lane);
+    }
+    const uint32_t kept = __ballot_sync(kAll, lane < a.n_group && rank < a.topk_group);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (e0 + j < a.E && !((kept >> ((e0 + j) / G)) & 1u)) live &= ~(1u << j);
+  }
+  int pick = -1;
+  for (int k = 0; k < a.K; ++k) {
+    double best = (double)neg_inf();
+    int at = INT_MAX;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (((live >> j) & 1u) && (at == INT_MAX || c[j] > best)) {
+        best = c[j];
+        at = e0 + j;
+      }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const double pv = __shfl_xor_sync(kAll, best, o);
+      const int pe = __shfl_xor_sync(kAll, at, o);
+      if (pv > best || (pv == best && pe < at)) {
+        best = pv;
+        at = pe;
+      }
+    }
+    if (at == INT_MAX) break;  // fewer usable experts than top_k
+    if (at / EPL == lane) live &= ~(1u << (at % EPL));
+    if (lane == k) pick = at;
+  }
+  return pick;
+}
+
+// The weights of the picked experts (lane k < K holds pick k) from their logits. For plain
+// softmax weights `top` and `sum` are those of the whole row.
+__device__ __forceinline__ float pick_weight(const RouterArgs& a, int pick, float x, float top,
+                                             float sum) {
+  if (a.softmax) {
+    if (a.renorm) {
+      const float m = warp_max(pick >= 0 ? x : neg_inf());
+      const float e = pick >= 0 ? exp_below_f(x, m) : 0.0f;
+      const float total = warp_sum(e);
+      return pick >= 0 ? e / total : 0.0f;
+    }
+    return pick >= 0 ? exp_below_f(x, top) / sum : 0.0f;
+  }
+  return pick >= 0 ? 1.0f / (1.0f + expf(-x)) : 0.0f;
+}
+
+template <int EPL>
+__device__ __forceinline__ void row_softmax(const float (&x)[EPL], float& top, float& sum) {
+  top = neg_inf();
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
+  top = warp_max(top);
+  sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) sum += x[j] > neg_inf() ? exp_below_f(x[j], top) : 0.0f;
+  sum = warp_sum(sum);
+}
+
+template <int EPL, typename In>
+__global__ void __launch_bounds__(kRouterWarps * 32) route_experts_kernel(RouterArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  float x[EPL];
+  load_logits<EPL, In>(a, t, lane, x);
+  const int pick = select_experts<EPL>(a, x, lane);
+  float top = 0.0f, sum = 1.0f;
+  if (a.softmax && !a.renorm) row_softmax<EPL>(x, top, sum);
+  const float xp =
+      pick >= 0 ? to_float(static_cast<const In*>(a.logits)[t * a.stride + pick]) : 0.0f;
+  float w = pick_weight(a, pick, xp, top, sum);
+  if (a.renorm && !a.softmax) {
+    const float total = warp_sum(w) + 1e-20f;
+    w = w / total;
+  }
+  if (lane < a.K) {
+    a.idx[t * a.K + lane] = pick;
+    a.w[t * a.K + lane] = w * a.scale;
+  }
+}
+
+// Gradient of the logits. With s the scores, g the gradient of the weights, p the
+// renormalised weights before the scale:
+//   softmax, renormalised   d_k = scale p_k (g_k - sum_m g_m p_m)        picked experts only
+//   softmax, plain          d_k = scale s_k g_k, dx_i = d_i - s_i sum_m d_m      every expert
+//   sigmoid, renormalised   d_k = scale / S (g_k - sum_m g_m s_m / S) s_k (1 - s_k)
+//   sigmoid, plain          d_k = scale g_k s_k (1 - s_k)
+// An expert named by several picks gets the sum of their terms.
+template <int EPL, typename In>
+__global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(RouterArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  const In* row = static_cast<const In*>(a.logits) + t * a.stride;
+  In* out = static_cast<In*>(a.grad_logits) + t * a.E;
+  int pick = lane < a.K ? a.idx[t * a.K + lane] : -1;
+  if (pick >= a.E || pick < 0) pick = -1;
+  const float xp = pick >= 0 ? to_float(row[pick]) : neg_inf();
+  if (!(xp > neg_inf())) pick = -1;
+  const float g = pick >= 0 ? a.grad_w[t * a.K + lane] : 0.0f;
+  const bool dense = a.softmax && !a.renorm;
+  float x[EPL];
+  float top = 0.0f, sum = 1.0f;
+  if (dense) {
+    load_logits<EPL, In>(a, t, lane, x);
+    row_softmax<EPL>(x, top, sum);
+  }
+  const float s = pick_weight(a, pick, xp, top, sum);
+  float d;
+  if (a.softmax && a.renorm) {
+    d = a.scale * s * (g - warp_sum(g * s));
+  } else if (dense) {
+    d = a.scale * s * g;
+  } else {
+    // s (1 - s) with 1 - s = 1 / (1 + exp(x)): no cancellation near 1
+    const float slope = pick >= 0 ? s / (1.0f + expf(xp)) : 0.0f;
+    if (a.renorm) {
+      const float total = warp_sum(s) + 1e-20f;
+      const float mean = warp_sum(g * s) / total;
+      d = a.scale / total * (g - mean) * slope;
+    } else {
+      d = a.scale * g * slope;
+    }
+  }
+  if (pick < 0) d = 0.0f;
+  const float all = dense ? warp_sum(d) : 0.0f;
+  const int e0 = lane * EPL;
+  float dx[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    dx[j] = dense && x[j] > neg_inf() ? -all * (exp_below_f(x[j], top) / sum) : 0.0f;
+  for (int k = 0; k < a.K; ++k) {
+    const int at = __shfl_sync(kAll, pick, k) - e0;
+    const float dk = __shfl_sync(kAll, d, k);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (at == j) dx[j] += dk;
+  }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    if (e0 + j < a.E) out[e0 + j] = from_float<In>(dx[j]);
+}
+
+// ------------------------------------------------------------------------------ host side
+int bad(const std::string& msg) {
+  set_last_error(msg);
+  return FMOE_ERR_VALUE;
+}
+
+int check_router(const fmoe_router* r) {
+  if (!r) return bad("router must not be NULL");
+  if (r->num_tokens < 0 || r->num_tokens > (int64_t)1 << 31)
+    return bad("num_tokens must be in [0, 2^31]");
+  if (r->num_experts < 1 || r->num_experts > kRouterMaxExperts)
+    return bad("num_experts must be in [1, 1024]");
+  if (r->n_group < 1 || r->n_group > 32 || r->num_experts % r->n_group != 0)
+    return bad("n_group must be in [1, 32] and divide num_experts");
+  if (r->topk_group < 1 || r->topk_group > r->n_group)
+    return bad("topk_group must be in [1, n_group]");
+  if (r->top_k < 1 || r->top_k > 32 ||
+      r->top_k > r->topk_group * (r->num_experts / r->n_group))
+    return bad("top_k must be in [1, 32] and fit in the kept groups");
+  if (r->score != FMOE_SCORE_SOFTMAX && r->score != FMOE_SCORE_SIGMOID)
+    return bad("score must be FMOE_SCORE_SOFTMAX or FMOE_SCORE_SIGMOID");
+  if (r->group_score != FMOE_GROUP_TOP2 && r->group_score != FMOE_GROUP_MAX)
+    return bad("group_score must be FMOE_GROUP_TOP2 or FMOE_GROUP_MAX");
+  if (r->logits_stride < r->num_experts)
+    return bad("logits_stride must be at least num_experts");
+  if (r->logits_dtype < FMOE_F32 || r->logits_dtype > FMOE_F16) {
+    set_last_error("logits_dtype must be FMOE_F32, FMOE_BF16 or FMOE_F16");
+    return FMOE_ERR_TYPE;
+  }
+  if (r->bias_dtype != FMOE_F32 && r->bias_dtype != FMOE_BF16) {
+    set_last_error("bias_dtype must be FMOE_F32 or FMOE_BF16");
+    return FMOE_ERR_TYPE;
+  }
+  return FMOE_OK;
+}
+
+RouterArgs router_args(const fmoe_router* r, const void* logits) {
+  RouterArgs a = {};
+  a.logits = logits;
+  a.stride = r->logits_stride;
+  a.bias_bf16 = r->bias_dtype == FMOE_BF16;
+  a.T = r->num_tokens;
+  a.E = r->num_experts;
+  a.K = r->top_k;
+  a.n_group = r->n_group;
+  a.topk_group = r->topk_group;
+  a.softmax = r->score == FMOE_SCORE_SOFTMAX;
+  a.group_max = r->group_score == FMOE_GROUP_MAX;
+  a.renorm = r->renormalize != 0;
+  a.scale = r->scale;
+  return a;
+}
+
+template <int EPL, typename In>
+void launch_router(const RouterArgs& a, bool backward, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((a.T + kRouterWarps - 1) / kRouterWarps);
+  if (backward)
+    route_experts_grad_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
+  else
+    route_experts_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
+}
+
+template <typename In>
+void launch_router(const RouterArgs& a, bool backward, cudaStream_t stream) {
+  if (a.E <= 32) launch_router<1, In>(a, backward, stream);
+  else if (a.E <= 64) launch_router<2, In>(a, backward, stream);
+  else if (a.E <= 128) launch_router<4, In>(a, backward, stream);
+  else if (a.E <= 256) launch_router<8, In>(a, backward, stream);
+  else if (a.E <= 512) launch_router<16, In>(a, backward, stream);
+  else launch_router<32, In>(a, backward, stream);
+}
+
+int launch_router(const fmoe_router* r, const RouterArgs& a, bool backward, cudaStream_t stream) {
+  if (r->logits_dtype == FMOE_F32) launch_router<float>(a, backward, stream);
+  else if (r->logits_dtype == FMOE_BF16) launch_router<__nv_bfloat16>(a, backward, stream);
+  else launch_router<__half>(a, backward, stream);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return FMOE_OK;
+  set_last_error(std::string("expert routing: ") + cudaGetErrorString(e));
+  return FMOE_ERR_RUNTIME;
+}
+
+}  // namespace
+}  // namespace fmoe
+
+using namespace fmoe;
+
+extern "C" int fmoe_route_experts(const fmoe_router* r, const void* logits, const void* bias,
+                                  const fmoe_route_out* out, void* stream) {
+  const int v = check_router(r);
+  if (v != FMOE_OK) return v;
+  if (r->num_tokens == 0) return FMOE_OK;
+  if (!logits || !out || !out->topk_idx || !out->topk_w)
+    return bad("routing pointers must not be NULL");
+  RouterArgs a = router_args(r, logits);
+  a.bias = bias;
+  a.idx = out->topk_idx;
+  a.w = out->topk_w;
+  return launch_router(r, a, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fmoe_route_experts_backward(const fmoe_router* r, const float* grad_w,
+                                           const void* logits, const int32_t* topk_idx,
+                                           void* grad_logits, void* stream) {
+  const int v = check_router(r);
+  if (v != FMOE_OK) return v;
+  if (r->num_tokens == 0) return FMOE_OK;
+  if (!logits || !grad_w || !topk_idx || !grad_logits)
+    return bad("routing pointers must not be NULL");
+  RouterArgs a = router_args(r, logits);
+  a.idx = const_cast<int*>(topk_idx);
+  a.grad_w = grad_w;
+  a.grad_logits = grad_logits;
+  return launch_router(r, a, true, static_cast<cudaStream_t>(stream));
+}

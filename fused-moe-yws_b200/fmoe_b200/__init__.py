@@ -40,7 +40,8 @@ EXPORTED_SYMBOLS = ("fmoe_abi_version", "fmoe_last_error", "fmoe_validate", "fmo
                     "fmoe_tile_n", "fmoe_prelayout_weights", "fmoe_forward_prelaid",
                     "fmoe_ep_plan_placed", "fmoe_forward_routed_count", "fmoe_ep_unpack_count",
                     "fmoe_ep_offsets", "fmoe_forward_routed_count_p2p",
-                    "fmoe_forward_routed_prelaid")
+                    "fmoe_forward_routed_prelaid", "fmoe_route_experts",
+                    "fmoe_route_experts_backward")
 
 
 class FmoeProblem(ctypes.Structure):
@@ -137,6 +138,8 @@ def load_library(path: Path | str | None = None):
         lib.fmoe_selftest_inject_device_error.argtypes = [ctypes.c_int32]
         lib.fmoe_probe_fp8_mma_rate.argtypes = [i64, ctypes.POINTER(ctypes.c_double),
                                                 ctypes.POINTER(ctypes.c_double), vp]
+        lib.fmoe_route_experts.argtypes = [vp, vp, vp, ctypes.POINTER(FmoeRouteOut), vp]
+        lib.fmoe_route_experts_backward.argtypes = [vp, vp, vp, vp, vp, vp]
         for name in EXPORTED_SYMBOLS:
             if not hasattr(lib, name):
                 raise RuntimeError(f"{p} does not export {name}")
@@ -781,3 +784,6 @@ def load_tvm_ffi_kernel():
         raise RuntimeError(f"TVM-FFI binding not built: {TVM_FFI_LIB_PATH}")
     mod = tvm_ffi.load_module(str(TVM_FFI_LIB_PATH))
     return mod["kernel"]
+
+
+from .router import route_experts, route_experts_backward  # noqa: E402,F401

@@ -330,6 +330,51 @@ int fmoe_ep_return_p2p(const void* partial, int64_t rows, int hidden_size, int w
                        const int64_t* src_start, void* const* peer_back, const int64_t* row_shift,
                        int64_t capacity_rows, int* err, void* stream);
 
+/* Element types of the entry points below. */
+enum fmoe_dtype { FMOE_F32 = 0, FMOE_BF16 = 1, FMOE_F16 = 2 };
+
+/* Expert routing for any scoring rule (fmoe_route serves the reference's one: sigmoid scores,
+ * a bf16 bias, groups, kernel.cu:388-516). With x the logits of a token:
+ *   s = softmax(x) or sigmoid(x); an expert whose logit is -inf or NaN is never picked and
+ *     has no share of the softmax;
+ *   c = s + bias (a bias of -inf also takes an expert out); without a bias the order of the
+ *     scores is the order of the logits;
+ *   of n_group groups of consecutive experts the topk_group best are kept, by the sum of their
+ *     two largest c (a group with fewer than two usable experts counts as -inf) or the largest;
+ *   topk_idx = the top_k experts of the kept groups by c, largest first, -1 where none is left;
+ *   topk_w = scale * s_k; with renormalize, scale * softmax over the picked experts, or for
+ *     the sigmoid scale * s_k / (sum of the picked s + 1e-20); 0 beside an index of -1.
+ * Every choice goes to the larger value in exact arithmetic and to the lower index on a tie.
+ * num_experts <= 1024, top_k and n_group <= 32. */
+enum fmoe_score { FMOE_SCORE_SOFTMAX = 0, FMOE_SCORE_SIGMOID = 1 };
+enum fmoe_group_score { FMOE_GROUP_TOP2 = 0, FMOE_GROUP_MAX = 1 };
+typedef struct fmoe_router {
+  int64_t num_tokens;
+  int64_t logits_stride; /* elements between the rows of logits, >= num_experts */
+  int32_t num_experts;
+  int32_t top_k;
+  int32_t n_group;
+  int32_t topk_group;
+  int32_t score;        /* fmoe_score */
+  int32_t group_score;  /* fmoe_group_score */
+  int32_t renormalize;
+  int32_t logits_dtype; /* fmoe_dtype */
+  int32_t bias_dtype;   /* FMOE_F32 or FMOE_BF16 */
+  float scale;
+} fmoe_router;
+
+/* logits [T, E] and bias [E] (or NULL) are device pointers, aligned to their type. No
+ * workspace; calls may overlap. */
+int fmoe_route_experts(const fmoe_router* r, const void* logits, const void* bias,
+                       const fmoe_route_out* out, void* stream);
+
+/* grad_logits [T, E] (the type of the logits, rows back to back, written completely) =
+ * d/dx sum_k grad_w[k] topk_w[k] for the picks topk_idx of fmoe_route_experts (grad_w and
+ * topk_idx [T, top_k]). The picks are held fixed, so the bias has no gradient. Indices outside
+ * [0, E) take no part; an expert named twice gets both terms. */
+int fmoe_route_experts_backward(const fmoe_router* r, const float* grad_w, const void* logits,
+                                const int32_t* topk_idx, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
