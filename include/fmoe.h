@@ -375,6 +375,49 @@ int fmoe_route_experts(const fmoe_router* r, const void* logits, const void* bia
 int fmoe_route_experts_backward(const fmoe_router* r, const float* grad_w, const void* logits,
                                 const int32_t* topk_idx, void* grad_logits, void* stream);
 
+/* Matrices of 4-bit blocks (the reference's weights are FP8 with 128 x 128 block scales,
+ * kernel.cu:781-782; these are half the bytes and multiply at twice the rate on sm_100a).
+ *   FMOE_MXFP4: 32 values share 2^e, e = floor(log2 of the largest magnitude) - 2, at least -127
+ *   FMOE_NVFP4: 16 values share the e4m3 number nearest to (largest magnitude / (6 g)), 448 at
+ *     most, where g is the matrix's fp32 global scale (positive; 1 without one); the block's
+ *     scale is that number times g
+ * A value divided by its block's scale (in fp32) is rounded to the nearest of 0, .5, 1, 1.5, 2,
+ * 3, 4, 6 (ties to the even code, 6 at most). A block that holds an infinity or a NaN has the
+ * scale NaN and stands for NaN.
+ *   codes  [batch, rows, cols / 2] bytes: two codes (sign, 2 exponent bits, 1 mantissa bit) a
+ *          byte, the value with the lower index in the low half
+ *   scales [batch, ceil(rows / 128), ceil(cols / (4 block)), 512] bytes: the byte of (row, block)
+ *          lies at (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of its tile; bytes past the
+ *          matrix's edge are zero
+ * Device pointers, 16-byte aligned. cols is a multiple of 32, at most 65536. */
+enum fmoe_fp4_format { FMOE_MXFP4 = 0, FMOE_NVFP4 = 1 };
+typedef struct fmoe_fp4_matrix {
+  void* codes;
+  void* scales;
+  const float* global_scale; /* [batch] on the device, or NULL */
+  int64_t rows;
+  int64_t cols;
+  int32_t batch;
+  int32_t format; /* fmoe_fp4_format */
+} fmoe_fp4_matrix;
+
+/* Bytes of the scales of a matrix with these sizes (its pointers are not read). */
+int fmoe_fp4_scale_bytes(const fmoe_fp4_matrix* q, size_t* bytes);
+
+/* Fills q's codes and scales from x: q->batch matrices, row r of matrix b at element
+ * b * batch_stride + r * row_stride; dtype is an fmoe_dtype. */
+int fmoe_fp4_quantize(const fmoe_fp4_matrix* q, const void* x, int32_t dtype, int64_t row_stride,
+                      int64_t batch_stride, void* stream);
+
+/* out [batch, rows, cols] (an fmoe_dtype, 16-byte aligned) = the values q stands for: the code
+ * times the block's scale in fp32, rounded to the type. */
+int fmoe_fp4_dequantize(const fmoe_fp4_matrix* q, void* out, int32_t dtype, void* stream);
+
+/* out [a->rows, b->rows] (an fmoe_dtype, 16-byte aligned) = a b^T, both of the same format and
+ * number of columns; summed in fp32, rounded once. Single matrices of at most 2^22 rows. */
+int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* b, void* out, int32_t dtype,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif
