@@ -283,6 +283,19 @@ int launch_route(const fmoe_problem* p, const Carved& c, const float* logits, co
 
 void fmoe::set_last_error(const std::string& msg) { g_last_error = msg; }
 
+int fmoe::num_sms() { return num_sms_current(); }
+
+unsigned* fmoe::device_error_sink(cudaStream_t stream) {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? error_sink_for(dev, stream) : nullptr;
+}
+
+int fmoe::make_byte_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
+                        uint32_t box_cols, uint32_t box_rows, const char* what) {
+  return make_map(map, base, cols, rows, cols, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
+                  what);
+}
+
 using namespace fmoe;
 
 extern "C" int fmoe_abi_version(void) { return FMOE_ABI_VERSION; }

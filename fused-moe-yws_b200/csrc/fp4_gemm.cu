@@ -1,7 +1,22 @@
-// fp4_gemm.cu -- products of 4-bit matrices.
+// fp4_gemm.cu -- products of 4-bit matrices on the tensor cores.
 //
-// out[m][n] = ga gb sum_k a[m][k] b[n][k], with a and b the codes times their block scales,
-// summed in fp32. One CTA per 64 x 64 tile, both operands decoded to fp32 in shared memory.
+// out[m][n] = ga gb sum_k a[m][k] b[n][k], a and b the codes times their block scales. The
+// sm_100a tensor core takes the codes from shared memory and the block scales from tensor
+// memory (tcgen05.mma block_scale), multiplies them into every product and sums in fp32, so
+// nothing is decoded and no partial sum leaves tensor memory before the last K step.
+//
+// A CTA (one per SM, persistent) computes tiles of 128 rows of a by BN rows of b. K steps of 256
+// values: 128 bytes of codes a row (one 128-byte swizzle row) and the scale tiles of those 256
+// columns, which lie back to back in memory (fp4.cuh). Warp 0 issues the copies, warp 1 the
+// scale copies into tensor memory and the MMAs (4 of K = 64 a step), warps 2..9 store tiles.
+// Scale columns in tensor memory have two slots: the copies for step k + 2 are issued when the
+// MMAs of step k have retired. A scale operand starts at a whole scale tile (4 columns), so BN
+// is a multiple of 128.
+//
+// Tensor memory has 512 columns. At BN = 128 two accumulators lie side by side. At BN = 256
+// two of them and the scales do not fit: the accumulators overlap by 96 columns, which the
+// epilogue reads first, and the next tile starts as soon as those are in registers.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -9,85 +24,430 @@
 #include <string>
 
 #include "fmoe.h"
+#include "fmoe_common.cuh"
 #include "fmoe_kernels.cuh"
 #include "fp4.cuh"
 #include "fp4_kernels.cuh"
+#include "sm100.cuh"
 
 namespace fmoe {
 namespace {
 
 using namespace fp4;
+using namespace sm100;
 
-struct ProductArgs {
-  const uint8_t *a, *b, *sa, *sb;
-  const float *ga, *gb;
-  int64_t M, N;
-  int K;
-  void* out;
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 8;
+constexpr int kStepCols = 256;      // K values per step
+constexpr int kABytes = 128 * 128;
+constexpr int kSmemLimit = 232448;
+constexpr int kOverlap = 96;        // columns two 256-column accumulators share
+
+template <int kFormat, int BN>
+struct Cfg {
+  static constexpr int kScaleTiles = kStepCols / tile_cols(kFormat);  // per 128 rows and step
+  static constexpr int kRunBytes = kScaleTiles * kTileBytes;
+  static constexpr int kRuns = BN / 128;                              // 128-row runs of b
+  static constexpr int kBBytes = BN * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes + (1 + kRuns) * kRunBytes;
+  static constexpr int kFixed = 1024 + 512;
+  static constexpr int kStagesRaw = (kSmemLimit - kFixed) / kStageBytes;
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
+  static constexpr int kSmemBytes = kFixed + kStages * kStageBytes;
+  // tensor memory
+  static constexpr bool kOverlapped = BN > 128;
+  static constexpr int kAcc1 = kOverlapped ? BN - kOverlap : BN;      // second accumulator
+  static constexpr int kScales = kAcc1 + BN;                          // first scale column
+  static constexpr int kSfaCols = kScaleTiles * 4;
+  static constexpr int kSlotCols = kSfaCols * (1 + kRuns);
+  static_assert(kScales + 2 * kSlotCols <= 512, "tensor memory budget");
+  static_assert(BN % 128 == 0, "scale operands start at whole scale tiles");
+  static_assert(kStages >= 3, "pipeline depth");
+  static_assert(kStageBytes % 1024 == 0, "stage alignment");
 };
 
-constexpr int kT = 64, kK = 32;
-
-template <int kFormat>
-__device__ __forceinline__ void stage(float (*s)[kT + 1], const uint8_t* codes,
-                                      const uint8_t* scales, int64_t r0, int64_t rows, int k0,
-                                      int K) {
-  // 64 rows x 32 columns: 256 threads, 8 values each
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-  float v[8] = {};
-  if (r0 + r < rows) {
-    const int64_t m = r0 + r;
-    decode8(*reinterpret_cast<const uint32_t*>(codes + m * (K / 2) + (k0 + c) / 2), v);
-    const int block = (k0 + c) / block_of(kFormat);
-    const int64_t tile = m / kTileRows * tiles_across(K, kFormat) + block / 4;
-    const float f = scale_value<kFormat>(
-        scales[tile * kTileBytes + scale_offset((int)(m % kTileRows), block)]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= f;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[c + i][r] = v[i];
+// scale tile (128 rows x 4 blocks) -> 4 tensor memory columns: lane l, column j holds the four
+// scale bytes of row 32 j + l
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
+  const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3FFF)  // start address
+                        | ((uint64_t)8 << 16) | ((uint64_t)8 << 32)  // 8-row groups 128 B apart
+                        | ((uint64_t)1 << 46);             // descriptor version; no swizzle
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
 }
 
-template <int kFormat, typename T>
-__global__ void __launch_bounds__(256) fp4_product_kernel(ProductArgs p) {
-  __shared__ float s_a[kK][kT + 1], s_b[kK][kT + 1];
-  const int64_t m0 = (int64_t)blockIdx.x * kT, n0 = (int64_t)blockIdx.y * kT;
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += kK) {
-    stage<kFormat>(s_a, p.a, p.sa, m0, p.M, k0, p.K);
-    stage<kFormat>(s_b, p.b, p.sb, n0, p.N, k0, p.K);
-    __syncthreads();
-#pragma unroll 8
-    for (int k = 0; k < kK; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = fmaf(s_a[k][tm + 16 * i], s_b[k][tn + 16 * j], acc[i][j]);
-    __syncthreads();
+template <int kFormat>
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  if constexpr (kFormat == FMOE_MXFP4) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
+        "[%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
+        "[%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
   }
-  const float g = (p.ga ? *p.ga : 1.0f) * (p.gb ? *p.gb : 1.0f);
+}
+
+// Instruction descriptor: e2m1 x e2m1 -> fp32, K-major, 128 x N x 64. mxfp4: the MMA's two
+// scales are bytes `half` and `half + 1` of the four in the column.
+template <int kFormat>
+__device__ __forceinline__ uint32_t idesc_fp4(int n, int half) {
+  return (1u << 7) | (1u << 10)                              // A, B = e2m1
+         | ((uint32_t)half << 4) | ((uint32_t)half << 29)    // scale bytes of B, of A
+         | ((uint32_t)(n >> 3) << 17)                        // N / 8
+         | (kFormat == FMOE_MXFP4 ? 1u << 23 : 0u)           // scales are e8m0 (else e4m3)
+         | (1u << 27);                                       // M / 128
+}
+
+struct Tile {
+  int64_t m0;   // first row of a
+  int rows;     // rows present
+  int n0;       // first row of b
+};
+
+struct GemmFp4Args {
+  const uint8_t* sa;
+  const uint8_t* sb;
+  const float* ga;
+  const float* gb;
+  void* out;
+  int64_t M;
+  int N, K;
+  int m_tiles, n_tiles, panel;  // tiles in panels of `panel` row tiles, rows first
+  int dtype;
+  unsigned* sink;
+};
+
+__device__ __forceinline__ bool tile_of(const GemmFp4Args& p, int64_t i, int bn, Tile& t) {
+  if (i >= (int64_t)p.m_tiles * p.n_tiles) return false;
+  const int64_t per = (int64_t)p.panel * p.n_tiles;
+  const int first = (int)(i / per) * p.panel;
+  const int high = min(p.panel, p.m_tiles - first);
+  const int r = (int)(i % per);
+  t.m0 = (int64_t)(first + r % high) * 128;
+  t.n0 = r / high * bn;
+  t.rows = (int)min((int64_t)128, p.M - t.m0);
+  return true;
+}
+
+// 32 consecutive values of a row, from column n.
+__device__ __forceinline__ void store32(const GemmFp4Args& p, int64_t m, int n,
+                                        const uint32_t (&v)[32], float alpha, bool wide) {
+  const int64_t at = m * p.N + n;
+  if (wide && n + 32 <= p.N) {
+    if (p.dtype == FMOE_F32) {
+      float* o = static_cast<float*>(p.out) + at;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 32; i += 8) {
+        uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-      if (m < p.M && n < p.N) static_cast<T*>(p.out)[m * p.N + n] = (T)(acc[i][j] * g);
+        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(__uint_as_float(v[i + j]) * alpha);
+        st_global_v8(o + i, w);
+      }
+    } else {
+      uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = __uint_as_float(v[i + 2 * j]) * alpha;
+          const float y = __uint_as_float(v[i + 2 * j + 1]) * alpha;
+          if (p.dtype == FMOE_BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            const __half2 h = __floats2half2_rn(x, y);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        st_global_v8(o + i, w);
+      }
     }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (n + i >= p.N) break;
+    const float x = __uint_as_float(v[i]) * alpha;
+    if (p.dtype == FMOE_F32) static_cast<float*>(p.out)[at + i] = x;
+    else if (p.dtype == FMOE_BF16) static_cast<__nv_bfloat16*>(p.out)[at + i] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(p.out)[at + i] = __float2half_rn(x);
+  }
+}
+
+template <int kFormat, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_b, const GemmFp4Args p) {
+  using C = Cfg<kFormat, BN>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stages + S * C::kStageBytes);
+  uint64_t* full = bars;         // [S] copies -> MMA
+  uint64_t* empty = bars + 8;    // [S] MMA -> copies
+  uint64_t* tfull = bars + 16;   // [2] MMA -> epilogue
+  uint64_t* tempty = bars + 18;  // [2] epilogue -> MMA
+  uint64_t* mma_done = bars + 20;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 22);
+  int* err = reinterpret_cast<int*>(bars + 23);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], kEpiWarps);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    *err = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int steps = (p.K + kStepCols - 1) / kStepCols;
+  const int across = tiles_across(p.K, kFormat);  // scale tiles per 128 rows
+  // how many tiles back the accumulator of a tile must have been read
+  constexpr int kBack = C::kOverlapped ? 1 : 2;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ copies
+      const uint64_t keep = policy_evict_last();
+      int it = 0;
+      bool ok = true;
+      Tile t;
+      for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x) {
+        const uint8_t* sa = p.sa + t.m0 / 128 * across * kTileBytes;
+        const uint8_t* sb = p.sb + (int64_t)(t.n0 / 128) * across * kTileBytes;
+        for (int k = 0; k < steps; ++k, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = stages + s * C::kStageBytes;
+          uint8_t* sc = st + kABytes + C::kBBytes;
+          const int have = min(C::kScaleTiles, across - k * C::kScaleTiles) * kTileBytes;
+          // runs of b past its last 128 rows do not exist
+          int runs = 1;
+          if constexpr (C::kRuns == 2) runs = t.n0 + 128 < p.N ? 2 : 1;
+          mbar_arrive_expect_tx(&full[s], kABytes + C::kBBytes + (1 + runs) * have);
+          tma_load_2d(st, &map_a, &full[s], k * 128, (int)t.m0, keep);
+          tma_load_2d(st + kABytes, &map_b, &full[s], k * 128, t.n0, keep);
+          const int64_t at = (int64_t)k * C::kScaleTiles * kTileBytes;
+          bulk_load_1d(sc, sa + at, have, &full[s]);
+          for (int r = 0; r < runs; ++r)
+            bulk_load_1d(sc + (1 + r) * C::kRunBytes,
+                         sb + (int64_t)r * across * kTileBytes + at, have, &full[s]);
+        }
+      }
+      if (!ok) {
+        atomicOr(err, kErrTimeoutProducer);
+        *abort_flag = 1;
+      }
+      // every issued copy must land before the CTA's shared memory is released
+      static const int zero = 0;
+      for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&full[j % S], (j / S) & 1, &zero);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ MMAs
+      int it = 0, n = 0;
+      bool ok = true;
+      Tile t;
+      for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x, ++n) {
+        if (n >= kBack &&
+            !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (n & 1) * C::kAcc1;
+        for (int k = 0; k < steps; ++k, ++it) {
+          const int s = it % S;
+          // the scale slot's last reader, two steps back
+          if ((it >= 2 && !mbar_wait(&empty[(it - 2) % S], ((it - 2) / S) & 1, abort_flag)) ||
+              !mbar_wait(&full[s], (it / S) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_addr(stages + s * C::kStageBytes);
+          const uint32_t sc = st + kABytes + C::kBBytes;
+          const uint32_t sfa = tmem + C::kScales + (it & 1) * C::kSlotCols;
+          const uint32_t sfb = sfa + C::kSfaCols;
+          const uint64_t ad = smem_desc_kmajor(st, 128);
+          const uint64_t bd = smem_desc_kmajor(st + kABytes, 128);
+          const int tiles = min(C::kScaleTiles, across - k * C::kScaleTiles);
+          for (int j = 0; j < tiles; ++j) {
+            copy_scales(sfa + 4 * j, sc + j * kTileBytes);
+#pragma unroll
+            for (int r = 0; r < C::kRuns; ++r)
+              copy_scales(sfb + 4 * (j * C::kRuns + r),
+                          sc + (1 + r) * C::kRunBytes + j * kTileBytes);
+          }
+          const int mmas = min(4, (p.K - k * kStepCols + 63) / 64);
+          for (int q = 0; q < mmas; ++q) {
+            const int j = kFormat == FMOE_MXFP4 ? q / 2 : q;
+            const int half = kFormat == FMOE_MXFP4 ? (q & 1) * 2 : 0;
+            mma_fp4<kFormat>(d, ad + 2 * q, bd + 2 * q, idesc_fp4<kFormat>(BN, half), sfa + 4 * j,
+                             sfb + 4 * j * C::kRuns, (k | q) != 0);
+          }
+          tc_commit(&empty[s]);
+        }
+        if (ok) tc_commit(&tfull[n & 1]);
+      }
+      if (!ok) {
+        atomicOr(err, kErrTimeoutMma);
+        *abort_flag = 1;
+      }
+      // all issued MMAs must retire before tensor memory is released
+      static const int zero = 0;
+      tc_commit(mma_done);
+      mbar_wait(mma_done, 0, &zero);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------------- epilogue
+    const int q = warp & 3;                   // tensor memory lanes 32 q .. 32 q + 31
+    const int half = (warp - 2) >> 2;         // columns half * BN / 2 ..
+    const float alpha = (p.ga ? *p.ga : 1.0f) * (p.gb ? *p.gb : 1.0f);
+    const bool wide = (int64_t)p.N * (p.dtype == FMOE_F32 ? 4 : 2) % 32 == 0 &&
+                      reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+    constexpr int kChunks = BN / 64;          // 32-column chunks of this warp
+    int n = 0;
+    bool ok = true;
+    Tile t;
+    for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x, ++n) {
+      if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + (n & 1) * C::kAcc1 + ((uint32_t)(q * 32) << 16);
+      const int row = q * 32 + lane;
+      const int64_t m = t.m0 + row;
+      if constexpr (!C::kOverlapped) {
+        const uint32_t col = half * (BN / 2);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32b<32>(acc + col + 32 * c, v);
+          tmem_ld_wait();
+          if (c == kChunks - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[n & 1]);
+          }
+          if (row < t.rows) store32(p, m, t.n0 + col + 32 * c, v, alpha, wide);
+        }
+      } else {
+        // the columns that the next tile's accumulator shares with this one come first:
+        // 160..255 of the first accumulator (upper half's 32..127), 0..95 of the second (lower
+        // half's 0..95)
+        const bool first = (n & 1) == 0;
+        const uint32_t col = half * 128;
+        const bool shares = first == (half == 1);
+        const uint32_t c0 = col + (shares && first ? 32 : 0);
+        uint32_t v0[32], v1[32], v2[32];
+        if (shares) {
+          tmem_ld_32x32b<32>(acc + c0, v0);
+          tmem_ld_32x32b<32>(acc + c0 + 32, v1);
+          tmem_ld_32x32b<32>(acc + c0 + 64, v2);
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[n & 1]);
+        if (shares) {
+          if (row < t.rows) {
+            store32(p, m, t.n0 + c0, v0, alpha, wide);
+            store32(p, m, t.n0 + c0 + 32, v1, alpha, wide);
+            store32(p, m, t.n0 + c0 + 64, v2, alpha, wide);
+          }
+          const uint32_t c1 = first ? col : col + 96;
+          tmem_ld_32x32b<32>(acc + c1, v0);
+          tmem_ld_wait();
+          if (row < t.rows) store32(p, m, t.n0 + c1, v0, alpha, wide);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_32x32b<32>(acc + col + 32 * c, v0);
+            tmem_ld_wait();
+            if (row < t.rows) store32(p, m, t.n0 + col + 32 * c, v0, alpha, wide);
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      atomicOr(err, kErrTimeoutEpilogue);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *err != 0 && p.sink) report_device_error(p.sink, *err);
+}
+
+template <int kFormat, int BN>
+cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const GemmFp4Args& p, int grid,
+                   cudaStream_t stream) {
+  auto* fn = fp4_gemm_kernel<kFormat, BN>;
+  static thread_local int configured = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (configured != dev) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<kFormat, BN>::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    configured = dev;
+  }
+  return launch_pdl(fn, dim3((unsigned)grid), dim3(kThreads), Cfg<kFormat, BN>::kSmemBytes, stream,
+                    a, b, p);
 }
 
 template <int kFormat>
-cudaError_t product(const ProductArgs& p, int dtype, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.M + kT - 1) / kT), (unsigned)((p.N + kT - 1) / kT));
-  if (dtype == FMOE_F32)
-    fp4_product_kernel<kFormat, float><<<grid, 256, 0, stream>>>(p);
-  else if (dtype == FMOE_BF16)
-    fp4_product_kernel<kFormat, __nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-  else
-    fp4_product_kernel<kFormat, __half><<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch(int bn, const CUtensorMap& a, const CUtensorMap& b, const GemmFp4Args& p,
+                   int grid, cudaStream_t stream) {
+  if (bn == 128) return launch<kFormat, 128>(a, b, p, grid, stream);
+  return launch<kFormat, 256>(a, b, p, grid, stream);
 }
 
 int bad(const std::string& msg) {
@@ -101,7 +461,7 @@ int bad(const std::string& msg) {
 using namespace fmoe;
 
 extern "C" int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* b, void* out,
-                               int32_t dtype, void* stream) {
+                               int32_t dtype, void* stream_ptr) {
   int v = fp4_check(a, "a");
   if (v != FMOE_OK) return v;
   if ((v = fp4_check(b, "b")) != FMOE_OK) return v;
@@ -118,12 +478,32 @@ extern "C" int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* 
   if ((v = fp4_check_pointers(a, "a")) != FMOE_OK) return v;
   if ((v = fp4_check_pointers(b, "b")) != FMOE_OK) return v;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16) return bad("out must be 16-byte aligned");
-  ProductArgs p = {static_cast<const uint8_t*>(a->codes), static_cast<const uint8_t*>(b->codes),
-                   static_cast<const uint8_t*>(a->scales), static_cast<const uint8_t*>(b->scales),
-                   a->global_scale, b->global_scale, a->rows, b->rows, (int)a->cols, out};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->format == FMOE_MXFP4 ? product<FMOE_MXFP4>(p, dtype, s)
-                                                : product<FMOE_NVFP4>(p, dtype, s);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const int sms = num_sms();
+  GemmFp4Args p = {};
+  p.sa = static_cast<const uint8_t*>(a->scales);
+  p.sb = static_cast<const uint8_t*>(b->scales);
+  p.ga = a->global_scale;
+  p.gb = b->global_scale;
+  p.out = out;
+  p.M = a->rows;
+  p.N = (int)b->rows;
+  p.K = (int)a->cols;
+  p.dtype = dtype;
+  p.m_tiles = (int)fp4::tiles_down(p.M);
+  // the widest tile that still gives every SM one
+  int bn = 256;
+  while (bn > 128 && (int64_t)p.m_tiles * ((p.N + bn - 1) / bn) < sms) bn /= 2;
+  p.n_tiles = (p.N + bn - 1) / bn;
+  p.panel = 8;
+  p.sink = device_error_sink(stream);
+  CUtensorMap ma, mb;
+  if ((v = make_byte_map(&ma, a->codes, p.K / 2, p.M, 128, 128, "a")) != FMOE_OK) return v;
+  if ((v = make_byte_map(&mb, b->codes, p.K / 2, p.N, 128, bn, "b")) != FMOE_OK) return v;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int grid = (int)(tiles < sms ? tiles : sms);
+  const cudaError_t e = a->format == FMOE_MXFP4 ? launch<FMOE_MXFP4>(bn, ma, mb, p, grid, stream)
+                                                : launch<FMOE_NVFP4>(bn, ma, mb, p, grid, stream);
   if (e == cudaSuccess) return FMOE_OK;
   set_last_error(std::string("4-bit product: ") + cudaGetErrorString(e));
   return FMOE_ERR_RUNTIME;

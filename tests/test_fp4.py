@@ -139,7 +139,8 @@ def _close(got, a, b, dtype):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("M,N,K", [
     (1, 1, 32), (1, 128, 256), (7, 40, 64), (16, 4096, 512), (33, 129, 96), (128, 256, 1024),
-    (129, 255, 2080), (300, 300, 288), (1, 5000, 7168), (257, 1, 160), (64, 520, 4128)])
+    (129, 255, 2080), (300, 300, 288), (1, 5000, 7168), (257, 1, 160), (64, 520, 4128),
+    (1500, 3400, 1056), (4999, 1057, 288), (200, 19000, 544)])
 def test_matmul(fmoe, fmt, M, N, K):
     ca, sa, a = _operand(M, K, fmt, None, M + K)
     cb, sb, b = _operand(N, K, fmt, None, N + K + 1)
