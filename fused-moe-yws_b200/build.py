@@ -30,7 +30,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompil
               f"-I{INCLUDE}", "-Xptxas", "-v"]
 CU_SOURCES = ["route.cu", "permute.cu", "gemm_sm100.cu", "gemm_sm100_tm.cu", "fmoe_api.cu", "ep.cu",
               "route_static.cu", "selftest.cu", "route_experts.cu",
-              "fp4_quant.cu", "fp4_gemm.cu"]
+              "fp4_quant.cu", "fp4_gemm.cu", "fp4_moe.cu"]
 
 
 def _stale(target: Path, deps) -> bool:

@@ -291,9 +291,12 @@ unsigned* fmoe::device_error_sink(cudaStream_t stream) {
 }
 
 int fmoe::make_byte_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
-                        uint32_t box_cols, uint32_t box_rows, const char* what) {
-  return make_map(map, base, cols, rows, cols, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
-                  what);
+                        uint64_t batch, uint32_t box_cols, uint32_t box_rows, const char* what) {
+  const cuuint64_t dims[3] = {cols, rows, batch};
+  const cuuint64_t strides[2] = {cols, rows * cols};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1};
+  return encode_map(map, base, batch ? 3 : 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                    what);
 }
 
 using namespace fmoe;

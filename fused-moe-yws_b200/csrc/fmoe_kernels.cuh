@@ -156,11 +156,11 @@ cudaError_t launch_prelayout(const uint8_t* w13, const uint8_t* w2, uint8_t* w13
 void set_last_error(const std::string& msg);  // message returned by fmoe_last_error()
 // Host helpers of fmoe_api.cu for the other entry points: SMs of the current device; its error
 // sink (null where none can be made, see report_device_error); a 128-byte-swizzled tensor map
-// of a byte matrix [rows, cols] with boxes of box_rows x box_cols.
+// of byte matrices [batch, rows, cols] with boxes of box_rows x box_cols (rank 2 for batch 0).
 int num_sms();
 unsigned* device_error_sink(cudaStream_t stream);
 int make_byte_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
-                  uint32_t box_cols, uint32_t box_rows, const char* what);
+                  uint64_t batch, uint32_t box_cols, uint32_t box_rows, const char* what);
 size_t gemm_partial_bytes();
 
 }  // namespace fmoe

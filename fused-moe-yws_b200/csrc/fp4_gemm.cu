@@ -110,10 +110,13 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, int half) {
 }
 
 struct Tile {
-  int64_t m0;   // first row of a
+  int m;        // row tile of a
   int rows;     // rows present
   int n0;       // first row of b
+  int e;        // matrix of b
 };
+
+constexpr int kMaxExperts = 1024;
 
 struct GemmFp4Args {
   const uint8_t* sa;
@@ -123,20 +126,46 @@ struct GemmFp4Args {
   void* out;
   int64_t M;
   int N, K;
-  int m_tiles, n_tiles, panel;  // tiles in panels of `panel` row tiles, rows first
+  int m_tiles, n_tiles, panel;  // dense: tiles in panels of `panel` row tiles, rows first
   int dtype;
+  int experts;                  // grouped: > 0
+  const int* tile_first;
+  const int* count;
+  const float* row_w;
   unsigned* sink;
 };
 
-__device__ __forceinline__ bool tile_of(const GemmFp4Args& p, int64_t i, int bn, Tile& t) {
-  if (i >= (int64_t)p.m_tiles * p.n_tiles) return false;
-  const int64_t per = (int64_t)p.panel * p.n_tiles;
-  const int first = (int)(i / per) * p.panel;
-  const int high = min(p.panel, p.m_tiles - first);
-  const int r = (int)(i % per);
-  t.m0 = (int64_t)(first + r % high) * 128;
-  t.n0 = r / high * bn;
-  t.rows = (int)min((int64_t)128, p.M - t.m0);
+// Tile i of the launch. Grouped (first / count: the experts' row tiles and rows in shared
+// memory): an expert's tiles follow one another, its row tiles first, so that CTAs that run
+// together read the same rows of b.
+__device__ __forceinline__ bool tile_of(const GemmFp4Args& p, const int* first, const int* count,
+                                        int64_t i, int bn, Tile& t) {
+  if (p.experts == 0) {
+    if (i >= (int64_t)p.m_tiles * p.n_tiles) return false;
+    const int64_t per = (int64_t)p.panel * p.n_tiles;
+    const int m = (int)(i / per) * p.panel;
+    const int high = min(p.panel, p.m_tiles - m);
+    const int r = (int)(i % per);
+    t.m = m + r % high;
+    t.n0 = r / high * bn;
+    t.rows = (int)min((int64_t)128, p.M - (int64_t)t.m * 128);
+    t.e = 0;
+    return true;
+  }
+  if (i >= (int64_t)first[p.experts] * p.n_tiles) return false;
+  const int r = (int)(i / p.n_tiles);
+  int low = 0, high = p.experts;  // first[low] <= r < first[high]
+  while (high - low > 1) {
+    const int mid = (low + high) / 2;
+    if (first[mid] <= r) low = mid;
+    else high = mid;
+  }
+  const int tiles = first[low + 1] - first[low];
+  const int j = (int)(i - (int64_t)first[low] * p.n_tiles);
+  t.e = low;
+  t.m = first[low] + j % tiles;
+  t.n0 = j / tiles * bn;
+  t.rows = min(128, count[low] - j % tiles * 128);
   return true;
 }
 
@@ -191,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b, const GemmFp4Args p) {
   using C = Cfg<kFormat, BN>;
+  __shared__ int s_first[kMaxExperts + 1], s_count[kMaxExperts];
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>(
@@ -232,6 +262,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();
+  if (p.experts > 0) {
+    for (int e = threadIdx.x; e <= p.experts; e += kThreads) {
+      s_first[e] = p.tile_first[e];
+      if (e < p.experts) s_count[e] = p.count[e];
+    }
+    __syncthreads();
+  }
 
   const int steps = (p.K + kStepCols - 1) / kStepCols;
   const int across = tiles_across(p.K, kFormat);  // scale tiles per 128 rows
@@ -245,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       bool ok = true;
       Tile t;
-      for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x) {
-        const uint8_t* sa = p.sa + t.m0 / 128 * across * kTileBytes;
-        const uint8_t* sb = p.sb + (int64_t)(t.n0 / 128) * across * kTileBytes;
+      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x) {
+        const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
+        const uint8_t* sb = p.sb + ((int64_t)t.e * tiles_down(p.N) + t.n0 / 128) * across * kTileBytes;
         for (int k = 0; k < steps; ++k, ++it) {
           const int s = it % S;
           if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
@@ -261,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           int runs = 1;
           if constexpr (C::kRuns == 2) runs = t.n0 + 128 < p.N ? 2 : 1;
           mbar_arrive_expect_tx(&full[s], kABytes + C::kBBytes + (1 + runs) * have);
-          tma_load_2d(st, &map_a, &full[s], k * 128, (int)t.m0, keep);
-          tma_load_2d(st + kABytes, &map_b, &full[s], k * 128, t.n0, keep);
+          tma_load_2d(st, &map_a, &full[s], k * 128, t.m * 128, keep);
+          tma_load_3d(st + kABytes, &map_b, &full[s], k * 128, t.n0, t.e, keep);
           const int64_t at = (int64_t)k * C::kScaleTiles * kTileBytes;
           bulk_load_1d(sc, sa + at, have, &full[s]);
           for (int r = 0; r < runs; ++r)
@@ -285,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0, n = 0;
       bool ok = true;
       Tile t;
-      for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x, ++n) {
+      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
         if (n >= kBack &&
             !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag)) {
           ok = false;
@@ -341,14 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------------- epilogue
     const int q = warp & 3;                   // tensor memory lanes 32 q .. 32 q + 31
     const int half = (warp - 2) >> 2;         // columns half * BN / 2 ..
-    const float alpha = (p.ga ? *p.ga : 1.0f) * (p.gb ? *p.gb : 1.0f);
+    const float ga = p.ga ? *p.ga : 1.0f;
     const bool wide = (int64_t)p.N * (p.dtype == FMOE_F32 ? 4 : 2) % 32 == 0 &&
                       reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
     constexpr int kChunks = BN / 64;          // 32-column chunks of this warp
     int n = 0;
     bool ok = true;
     Tile t;
-    for (int64_t i = blockIdx.x; ok && tile_of(p, i, BN, t); i += gridDim.x, ++n) {
+    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
       if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
         ok = false;
         break;
@@ -356,7 +393,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1) * C::kAcc1 + ((uint32_t)(q * 32) << 16);
       const int row = q * 32 + lane;
-      const int64_t m = t.m0 + row;
+      const int64_t m = (int64_t)t.m * 128 + row;
+      float alpha = p.gb ? ga * p.gb[t.e] : ga;
+      if (p.row_w && row < t.rows) alpha *= p.row_w[m];
       if constexpr (!C::kOverlapped) {
         const uint32_t col = half * (BN / 2);
 #pragma unroll
@@ -456,12 +495,50 @@ int bad(const std::string& msg) {
 }
 
 }  // namespace
+
+int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
+  const int sms = num_sms();
+  GemmFp4Args p = {};
+  p.sa = static_cast<const uint8_t*>(g.sa);
+  p.sb = static_cast<const uint8_t*>(g.sb);
+  p.ga = g.ga;
+  p.gb = g.gb;
+  p.out = g.out;
+  p.M = g.M;
+  p.N = g.N;
+  p.K = g.K;
+  p.dtype = g.dtype;
+  p.experts = g.experts;
+  p.tile_first = g.tile_first;
+  p.count = g.count;
+  p.row_w = g.row_w;
+  p.m_tiles = (int)tiles_down(g.M);
+  // the widest tile that still gives every SM one
+  int bn = 256;
+  while (bn > 128 && (int64_t)p.m_tiles * ((g.N + bn - 1) / bn) < sms) bn /= 2;
+  p.n_tiles = (g.N + bn - 1) / bn;
+  p.panel = 8;
+  p.sink = device_error_sink(stream);
+  CUtensorMap ma, mb;
+  int v = make_byte_map(&ma, g.a, g.K / 2, g.M, 0, 128, 128, "a");
+  if (v == FMOE_OK)
+    v = make_byte_map(&mb, g.b, g.K / 2, g.N, g.experts > 0 ? g.experts : 1, 128, bn, "b");
+  if (v != FMOE_OK) return v;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int grid = (int)(tiles < sms ? tiles : sms);
+  const cudaError_t e = g.format == FMOE_MXFP4 ? launch<FMOE_MXFP4>(bn, ma, mb, p, grid, stream)
+                                               : launch<FMOE_NVFP4>(bn, ma, mb, p, grid, stream);
+  if (e == cudaSuccess) return FMOE_OK;
+  set_last_error(std::string("4-bit product: ") + cudaGetErrorString(e));
+  return FMOE_ERR_RUNTIME;
+}
+
 }  // namespace fmoe
 
 using namespace fmoe;
 
 extern "C" int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* b, void* out,
-                               int32_t dtype, void* stream_ptr) {
+                               int32_t dtype, void* stream) {
   int v = fp4_check(a, "a");
   if (v != FMOE_OK) return v;
   if ((v = fp4_check(b, "b")) != FMOE_OK) return v;
@@ -478,33 +555,18 @@ extern "C" int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* 
   if ((v = fp4_check_pointers(a, "a")) != FMOE_OK) return v;
   if ((v = fp4_check_pointers(b, "b")) != FMOE_OK) return v;
   if (!out || reinterpret_cast<uintptr_t>(out) % 16) return bad("out must be 16-byte aligned");
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const int sms = num_sms();
-  GemmFp4Args p = {};
-  p.sa = static_cast<const uint8_t*>(a->scales);
-  p.sb = static_cast<const uint8_t*>(b->scales);
-  p.ga = a->global_scale;
-  p.gb = b->global_scale;
-  p.out = out;
-  p.M = a->rows;
-  p.N = (int)b->rows;
-  p.K = (int)a->cols;
-  p.dtype = dtype;
-  p.m_tiles = (int)fp4::tiles_down(p.M);
-  // the widest tile that still gives every SM one
-  int bn = 256;
-  while (bn > 128 && (int64_t)p.m_tiles * ((p.N + bn - 1) / bn) < sms) bn /= 2;
-  p.n_tiles = (p.N + bn - 1) / bn;
-  p.panel = 8;
-  p.sink = device_error_sink(stream);
-  CUtensorMap ma, mb;
-  if ((v = make_byte_map(&ma, a->codes, p.K / 2, p.M, 128, 128, "a")) != FMOE_OK) return v;
-  if ((v = make_byte_map(&mb, b->codes, p.K / 2, p.N, 128, bn, "b")) != FMOE_OK) return v;
-  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int grid = (int)(tiles < sms ? tiles : sms);
-  const cudaError_t e = a->format == FMOE_MXFP4 ? launch<FMOE_MXFP4>(bn, ma, mb, p, grid, stream)
-                                                : launch<FMOE_NVFP4>(bn, ma, mb, p, grid, stream);
-  if (e == cudaSuccess) return FMOE_OK;
-  set_last_error(std::string("4-bit product: ") + cudaGetErrorString(e));
-  return FMOE_ERR_RUNTIME;
+  Fp4Gemm g = {};
+  g.format = a->format;
+  g.a = a->codes;
+  g.sa = a->scales;
+  g.M = a->rows;
+  g.b = b->codes;
+  g.sb = b->scales;
+  g.N = (int)b->rows;
+  g.K = (int)a->cols;
+  g.ga = a->global_scale;
+  g.gb = b->global_scale;
+  g.out = out;
+  g.dtype = dtype;
+  return launch_fp4_gemm(g, static_cast<cudaStream_t>(stream));
 }

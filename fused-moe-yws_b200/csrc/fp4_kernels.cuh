@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "fmoe.h"
+#include "fp4.cuh"
 
 namespace fmoe {
 
@@ -20,12 +21,37 @@ struct Fp4QuantArgs {
   uint8_t* codes;          // [batch, rows, cols / 2]
   uint8_t* scales;         // tiles, fp4.cuh
   const int* row_index;    // or null: row m is taken from x's row row_index[m]; below 0: none
-  const int* rows_dev;     // or null: row tiles from *rows_dev on are not touched
+  const int* tiles_dev;    // or null: row tiles from *tiles_dev on are not touched
+  bool swiglu;             // x is fp32 [rows, 2 cols], the value x[c] * silu(x[cols + c]) of the
+                           // same row; row_index only tells which rows there are
 };
 
 // Argument checks of one matrix: sizes and format; pointers.
 int fp4_check(const fmoe_fp4_matrix* q, const char* name);
 int fp4_check_pointers(const fmoe_fp4_matrix* q, const char* name);
+
+// A product out[m][n] = sum_k a[m][k] b[n][k]. Dense (experts == 0): M rows of a, one b.
+// Grouped: row tile r of a (128 rows) belongs to the expert e with tile_first[e] <= r <
+// tile_first[e + 1] and is multiplied by b's matrix e; an expert's count[e] rows fill its tiles
+// from the front, the rows behind them are not written.
+struct Fp4Gemm {
+  int format;
+  const void* a;          // codes [rows of a, K / 2]
+  const void* sa;
+  int64_t M;              // rows of a; grouped: its capacity, a multiple of 128
+  const void* b;          // codes [experts, N, K / 2]
+  const void* sb;
+  int N, K;
+  const float* ga;        // global scales or null; one per expert for b
+  const float* gb;
+  void* out;              // [M, N]
+  int dtype;
+  int experts;
+  const int* tile_first;  // [experts + 1] on the device
+  const int* count;       // [experts] on the device
+  const float* row_w;     // or null: factor of each row of out
+};
+int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream);
 
 cudaError_t launch_fp4_quantize(const Fp4QuantArgs& a, int format, int dtype, int batch,
                                 cudaStream_t stream);

@@ -63,7 +63,12 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
   }
 }
 
-template <int kFormat, typename T, bool kWide>
+// gate * silu(up) with the fast exponential and division: a few units in the last place
+__device__ __forceinline__ float swiglu(float gate, float up) {
+  return gate * __fdividef(up, 1.0f + __expf(-up));
+}
+
+template <int kFormat, typename T, bool kWide, bool kSwiglu = false>
 __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(Fp4QuantArgs a) {
   __shared__ __align__(16) uint8_t s_scale[kCols / tile_cols(kFormat) * kTileBytes];
   const int tid = threadIdx.x;
@@ -71,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(Fp4QuantArgs a) 
   const int c0 = blockIdx.y * kCols, e = blockIdx.z;
   pdl_wait();
   pdl_trigger();
-  if (a.rows_dev && m0 >= *a.rows_dev) return;  // row tiles nobody uses
+  if (a.tiles_dev && (int)blockIdx.x >= *a.tiles_dev) return;  // row tiles nobody uses
   const int across = tiles_across(a.cols, kFormat);
   const int first = c0 / tile_cols(kFormat);
   const int here = min(kCols / tile_cols(kFormat), across - first);
@@ -91,7 +96,15 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(Fp4QuantArgs a) 
     float v[16] = {};
     uint32_t top = 0;
     if (mine) {
-      load16<T, kWide>(x + src * a.row_stride + c, v);
+      if constexpr (kSwiglu) {
+        float up[16];
+        load16<T, kWide>(x + m * a.row_stride + c, v);
+        load16<T, kWide>(x + m * a.row_stride + a.cols + c, up);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = swiglu(v[i], up[i]);
+      } else {
+        load16<T, kWide>(x + src * a.row_stride + c, v);
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     }
@@ -182,6 +195,9 @@ cudaError_t quantize(const Fp4QuantArgs& a, int batch, cudaStream_t stream) {
 
 template <int kFormat>
 cudaError_t quantize(const Fp4QuantArgs& a, int dtype, int batch, cudaStream_t stream) {
+  if (a.swiglu)  // the expert layer's own fp32 buffer: aligned
+    return launch_pdl(fp4_quantize_kernel<kFormat, float, true, true>, grid_of(a, batch),
+                      dim3(kThreads), 0, stream, a);
   if (dtype == FMOE_F32) return quantize<kFormat, float>(a, batch, stream);
   if (dtype == FMOE_BF16) return quantize<kFormat, __nv_bfloat16>(a, batch, stream);
   return quantize<kFormat, __half>(a, batch, stream);

@@ -42,7 +42,8 @@ EXPORTED_SYMBOLS = ("fmoe_abi_version", "fmoe_last_error", "fmoe_validate", "fmo
                     "fmoe_ep_offsets", "fmoe_forward_routed_count_p2p",
                     "fmoe_forward_routed_prelaid", "fmoe_route_experts",
                     "fmoe_route_experts_backward", "fmoe_fp4_scale_bytes", "fmoe_fp4_quantize",
-                    "fmoe_fp4_dequantize", "fmoe_fp4_matmul")
+                    "fmoe_fp4_dequantize", "fmoe_fp4_matmul", "fmoe_fp4_workspace_size",
+                    "fmoe_fp4_forward")
 
 
 class FmoeProblem(ctypes.Structure):
@@ -145,6 +146,8 @@ def load_library(path: Path | str | None = None):
         lib.fmoe_fp4_quantize.argtypes = [vp, vp, ctypes.c_int32, i64, i64, vp]
         lib.fmoe_fp4_dequantize.argtypes = [vp, vp, ctypes.c_int32, vp]
         lib.fmoe_fp4_matmul.argtypes = [vp, vp, vp, ctypes.c_int32, vp]
+        lib.fmoe_fp4_workspace_size.argtypes = [vp, ctypes.POINTER(ctypes.c_size_t)]
+        lib.fmoe_fp4_forward.argtypes = [vp, vp, vp, ctypes.c_size_t, vp]
         for name in EXPORTED_SYMBOLS:
             if not hasattr(lib, name):
                 raise RuntimeError(f"{p} does not export {name}")
@@ -791,5 +794,6 @@ def load_tvm_ffi_kernel():
     return mod["kernel"]
 
 
-from .fp4 import Fp4Tensor, dequantize_fp4, matmul_fp4, quantize_fp4  # noqa: E402,F401
+from .fp4 import (Fp4Tensor, dequantize_fp4, forward_fp4, matmul_fp4,  # noqa: E402,F401
+                  quantize_fp4)
 from .router import route_experts, route_experts_backward  # noqa: E402,F401

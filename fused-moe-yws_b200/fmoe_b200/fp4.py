@@ -11,8 +11,8 @@ import dataclasses
 
 import torch
 
-from . import FMOE_OK, _check_tensor, _raise, load_library
-from .router import DTYPE_CODES
+from . import FMOE_OK, _raise, _raise_device_error, load_library
+from .router import DTYPE_CODES, _call, _expect
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
@@ -22,6 +22,19 @@ class FmoeFp4Matrix(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
                 ("global_scale", ctypes.c_void_p), ("rows", ctypes.c_int64),
                 ("cols", ctypes.c_int64), ("batch", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class FmoeFp4Problem(ctypes.Structure):
+    _fields_ = [("num_tokens", ctypes.c_int64), ("hidden_size", ctypes.c_int32),
+                ("intermediate_size", ctypes.c_int32), ("num_local_experts", ctypes.c_int32),
+                ("top_k", ctypes.c_int32), ("local_expert_offset", ctypes.c_int32),
+                ("format", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class FmoeFp4Tensors(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "hidden_states", "topk_idx", "topk_w", "w13", "w13_scales", "w13_global", "w2",
+        "w2_scales", "w2_global", "input_scale", "intermediate_scale", "output")]
 
 
 def _check_format(format):
@@ -81,37 +94,30 @@ class Fp4Tensor:
         _check_format(self.format)
         if not isinstance(self.codes, torch.Tensor) or self.codes.dim() not in dims:
             raise ValueError(f"{name}.codes must be {' or '.join(f'{d}D' for d in dims)}")
-        *lead, rows, half = self.codes.shape
-        _check_tensor(self.codes, f"{name}.codes", tuple(self.codes.shape), torch.uint8)
-        _check_tensor(self.scales, f"{name}.scales",
-                      _scale_shape(lead, rows, 2 * half, self.format), torch.uint8)
-        g = _global_scale(self.global_scale, lead, self.codes.device, f"{name}.global_scale",
-                          self.format)
-        if self.scales.device != self.codes.device:
-            raise ValueError(f"{name}.codes and {name}.scales must be on the same device")
-        return FmoeFp4Matrix(self.codes.data_ptr(), self.scales.data_ptr(), g, rows, 2 * half,
+        codes, dev = self.codes, self.codes.device
+        if dev.type != "cuda":
+            raise ValueError(f"{name}.codes must be a CUDA tensor")
+        *lead, rows, half = codes.shape
+        _expect(codes, f"{name}.codes", codes.shape, torch.uint8, dev)
+        _expect(self.scales, f"{name}.scales", _scale_shape(lead, rows, 2 * half, self.format),
+                torch.uint8, dev)
+        g = self.global_scale
+        if g is not None:
+            g = _global_scale(g, lead, dev, f"{name}.global_scale", self.format)
+        return FmoeFp4Matrix(codes.data_ptr(), self.scales.data_ptr(), g, rows, 2 * half,
                              lead[0] if lead else 1, FORMATS[self.format])
 
 
-def _global_scale(g, lead, device, name, format):
-    if g is None:
-        return None
+def _global_scale(g, lead, dev, name, format):
     if format == "mxfp4":
         raise ValueError(f"{name}: mxfp4 has no global scale")
-    if not isinstance(g, torch.Tensor) or g.device != device:
-        raise ValueError(f"{name} must be a tensor on {device}")
+    if not isinstance(g, torch.Tensor) or g.device != dev:
+        raise ValueError(f"{name} must be a tensor on {dev}")
     if g.numel() != (lead[0] if lead else 1) or not g.is_contiguous():
         raise ValueError(f"{name} must have one contiguous element per matrix")
-    if g.dtype != torch.float32:
+    if g.dtype is not torch.float32:
         raise TypeError(f"{name} dtype mismatch: expected torch.float32, got {g.dtype}")
     return g.data_ptr()
-
-
-def _call(lib, where, dev, fn, *args):
-    with torch.cuda.device(dev):
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    if rc != FMOE_OK:
-        _raise(lib, rc, where)
 
 
 def _out(out, shape, dtype, dev):
@@ -119,9 +125,7 @@ def _out(out, shape, dtype, dev):
         raise TypeError(f"output dtype mismatch: expected float32, bfloat16 or float16, got {dtype}")
     if out is None:
         return torch.empty(shape, dtype=dtype, device=dev)
-    _check_tensor(out, "out", tuple(shape), dtype)
-    if out.device != dev:
-        raise ValueError(f"out must be on {dev}")
+    _expect(out, "out", shape, dtype, dev)
     return out
 
 
@@ -154,8 +158,7 @@ def quantize_fp4(x: torch.Tensor, format: str, *, global_scale: torch.Tensor | N
     if lead and lead[0] == 0:
         return out
     q = out._matrix("out", (x.dim(),))
-    lib = load_library()
-    _call(lib, "quantize_fp4", dev, lib.fmoe_fp4_quantize, ctypes.byref(q), x.data_ptr(),
+    _call("quantize_fp4", dev, "fmoe_fp4_quantize", ctypes.byref(q), x.data_ptr(),
           DTYPE_CODES[x.dtype], x.stride(-2), x.stride(0) if lead else 0)
     return out
 
@@ -169,9 +172,8 @@ def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
     out = _out(out, q.shape, dtype, q.device)
     if out.numel() == 0:
         return out
-    lib = load_library()
-    _call(lib, "dequantize_fp4", q.device, lib.fmoe_fp4_dequantize, ctypes.byref(m),
-          out.data_ptr(), DTYPE_CODES[dtype])
+    _call("dequantize_fp4", q.device, "fmoe_fp4_dequantize", ctypes.byref(m), out.data_ptr(),
+          DTYPE_CODES[dtype])
     return out
 
 
@@ -182,10 +184,81 @@ def matmul_fp4(a: Fp4Tensor, b: Fp4Tensor, *, dtype: torch.dtype = torch.bfloat1
         if not isinstance(m, Fp4Tensor):
             raise ValueError(f"{name} must be an Fp4Tensor")
     ma, mb = a._matrix("a", (2,)), b._matrix("b", (2,))
-    if a.device != b.device:
+    if a.codes.device != b.codes.device:
         raise ValueError("a and b must be on the same device")
-    out = _out(out, (a.shape[0], b.shape[0]), dtype, a.device)
-    lib = load_library()
-    _call(lib, "matmul_fp4", a.device, lib.fmoe_fp4_matmul, ctypes.byref(ma), ctypes.byref(mb),
+    out = _out(out, (ma.rows, mb.rows), dtype, a.codes.device)
+    _call("matmul_fp4", a.device, "fmoe_fp4_matmul", ctypes.byref(ma), ctypes.byref(mb),
           out.data_ptr(), DTYPE_CODES[dtype])
+    return out
+
+
+def fp4_workspace_bytes(prob: FmoeFp4Problem) -> int:
+    lib = load_library()
+    n = ctypes.c_size_t(0)
+    rc = lib.fmoe_fp4_workspace_size(ctypes.byref(prob), ctypes.byref(n))
+    if rc != FMOE_OK:
+        _raise(lib, rc, "fp4_workspace_bytes")
+    return int(n.value)
+
+
+def forward_fp4(hidden_states: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
+                w13: Fp4Tensor, w2: Fp4Tensor, local_expert_offset: int = 0, *,
+                input_scale: torch.Tensor | None = None,
+                intermediate_scale: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None, check: bool = False) -> torch.Tensor:
+    """The expert layer on 4-bit weights; returns bf16 [T, H] (fmoe_fp4_forward).
+
+    ``hidden_states`` [T, H] (fp32, bf16 or fp16) are quantised by the call, ``topk_idx`` int32 /
+    ``topk_w`` fp32 [T, K] come from ``route_experts`` or ``route``. ``w13`` [E_local, 2I, H] (gate
+    rows, then up rows; the SiLU is on the up half, as in ``kernel``) and ``w2`` [E_local, H, I]
+    hold experts [offset, offset + E_local); picks outside take no part. ``input_scale`` and
+    ``intermediate_scale`` (nvfp4, fp32 [1] on the device) are the activations' global scales.
+    ``workspace`` is the caller's scratch (``fp4_workspace_bytes``; one call at a time), ``check``
+    as in ``kernel``; a device error of an earlier call raises ``DeviceError``."""
+    for name, m in (("w13", w13), ("w2", w2)):
+        if not isinstance(m, Fp4Tensor):
+            raise ValueError(f"{name} must be an Fp4Tensor")
+    if w13.format != w2.format:
+        raise ValueError("w13 and w2 must have the same format")
+    if not isinstance(hidden_states, torch.Tensor) or hidden_states.dim() != 2:
+        raise ValueError("hidden_states must be 2D")
+    if not isinstance(topk_idx, torch.Tensor) or topk_idx.dim() != 2:
+        raise ValueError("topk_idx must be 2D")
+    if hidden_states.dtype not in DTYPE_CODES:
+        raise TypeError(f"hidden_states dtype mismatch: expected float32, bfloat16 or float16, got "
+                        f"{hidden_states.dtype}")
+    m13, m2 = w13._matrix("w13", (3,)), w2._matrix("w2", (3,))
+    dev = w13.codes.device
+    T, K = topk_idx.shape
+    E, H, I = m13.batch, m13.cols, m13.rows // 2
+    if m13.rows % 2 or (m2.batch, m2.rows, m2.cols) != (E, H, I):
+        raise ValueError(f"w13 must be [E, 2I, H] and w2 [E, H, I], got {w13.shape} and {w2.shape}")
+    if w2.codes.device != dev:
+        raise ValueError("w13 and w2 must be on the same device")
+    _expect(hidden_states, "hidden_states", (T, H), hidden_states.dtype, dev)
+    _expect(topk_idx, "topk_idx", (T, K), torch.int32, dev)
+    _expect(topk_w, "topk_w", (T, K), torch.float32, dev)
+    scales = [None if g is None else _global_scale(g, [], dev, name, w13.format)
+              for name, g in (("input_scale", input_scale),
+                              ("intermediate_scale", intermediate_scale))]
+    prob = FmoeFp4Problem(T, H, I, E, K, int(local_expert_offset), m13.format,
+                          DTYPE_CODES[hidden_states.dtype])
+    nbytes = fp4_workspace_bytes(prob)
+    _raise_device_error(dev, "an earlier call on this device")
+    out = _out(out, (T, H), torch.bfloat16, dev)
+    if T == 0:
+        return out
+    if workspace is None:
+        # from the allocator, which orders it with this stream and keeps it for a capturing graph
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {dev}")
+    t = FmoeFp4Tensors(hidden_states.data_ptr(), topk_idx.data_ptr(), topk_w.data_ptr(),
+                       m13.codes, m13.scales, m13.global_scale, m2.codes, m2.scales,
+                       m2.global_scale, *scales, out.data_ptr())
+    _call("forward_fp4", dev, "fmoe_fp4_forward", ctypes.byref(prob), ctypes.byref(t),
+          workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    if check:
+        torch.cuda.current_stream(dev).synchronize()
+        _raise_device_error(dev, "this call")
     return out

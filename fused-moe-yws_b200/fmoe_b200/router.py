@@ -13,6 +13,10 @@ import torch
 
 from . import FMOE_OK, FmoeRouteOut, _check_tensor, _raise, load_library
 
+# the current stream's handle without a Stream object around it (half the host time of a call)
+_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"top2": 0, "max": 1}
@@ -31,6 +35,26 @@ def _code(table, value, name):
     if value not in table:
         raise ValueError(f"{name} must be one of {', '.join(table)}, got {value!r}")
     return table[value]
+
+
+def _expect(t, name, shape, dtype, dev):
+    """_check_tensor and the device, in one test for the arguments that are as they should be."""
+    if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype
+            and t.device == dev and t.is_contiguous()):
+        _check_tensor(t, name, shape, dtype)
+        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+
+
+def _call(where, dev, name, *args):
+    """The library's function `name` on dev's current stream; raises what it reports."""
+    lib = load_library()
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, _stream_handle(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(lib, name)(*args, _stream_handle(dev.index))
+    if rc != FMOE_OK:
+        _raise(lib, rc, where)
 
 
 def _logits(logits):
@@ -67,22 +91,15 @@ def _forward(logits, bias, top_k, score, n_group, topk_group, group_score, renor
         bias_dtype = bias.dtype
         if bias_dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"bias dtype mismatch: expected float32 or bfloat16, got {bias_dtype}")
-        _check_tensor(bias, "bias", (E,), bias_dtype)
-        if bias.device != logits.device:
-            raise ValueError("logits and bias must be on the same device")
+        _expect(bias, "bias", (E,), bias_dtype, logits.device)
     r = _router(logits, top_k, score, n_group, topk_group, group_score, renormalize, scale,
                 bias_dtype)
     dev = logits.device
     idx = torch.empty(T, max(int(top_k), 0), dtype=torch.int32, device=dev)
     w = torch.empty(T, max(int(top_k), 0), dtype=torch.float32, device=dev)
     out = FmoeRouteOut(idx.data_ptr(), w.data_ptr())
-    lib = load_library()
-    with torch.cuda.device(dev):
-        rc = lib.fmoe_route_experts(ctypes.byref(r), logits.data_ptr(),
-                                    bias.data_ptr() if bias is not None else None,
-                                    ctypes.byref(out), torch.cuda.current_stream(dev).cuda_stream)
-    if rc != FMOE_OK:
-        _raise(lib, rc, "route_experts")
+    _call("route_experts", dev, "fmoe_route_experts", ctypes.byref(r), logits.data_ptr(),
+          None if bias is None else bias.data_ptr(), ctypes.byref(out))
     return idx, w
 
 
@@ -98,24 +115,15 @@ def route_experts_backward(grad_w: torch.Tensor, logits: torch.Tensor, topk_idx:
     if not isinstance(topk_idx, torch.Tensor) or topk_idx.dim() != 2:
         raise ValueError("topk_idx must be 2D")
     K = topk_idx.shape[1]
-    _check_tensor(topk_idx, "topk_idx", (T, K), torch.int32)
-    if not isinstance(grad_w, torch.Tensor):
-        raise ValueError("grad_w must be a torch.Tensor")
-    grad_w = grad_w.contiguous()  # a gradient may arrive broadcast
-    _check_tensor(grad_w, "grad_w", (T, K), torch.float32)
-    for name, t in (("topk_idx", topk_idx), ("grad_w", grad_w)):
-        if t.device != logits.device:
-            raise ValueError(f"logits and {name} must be on the same device")
-    r = _router(logits, K, score, 1, 1, "top2", renormalize, scale)
     dev = logits.device
+    _expect(topk_idx, "topk_idx", (T, K), torch.int32, dev)
+    if isinstance(grad_w, torch.Tensor):
+        grad_w = grad_w.contiguous()  # a gradient may arrive broadcast
+    _expect(grad_w, "grad_w", (T, K), torch.float32, dev)
+    r = _router(logits, K, score, 1, 1, "top2", renormalize, scale)
     out = torch.empty(T, E, dtype=logits.dtype, device=dev)
-    lib = load_library()
-    with torch.cuda.device(dev):
-        rc = lib.fmoe_route_experts_backward(
-            ctypes.byref(r), grad_w.data_ptr(), logits.data_ptr(), topk_idx.data_ptr(),
-            out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    if rc != FMOE_OK:
-        _raise(lib, rc, "route_experts_backward")
+    _call("route_experts_backward", dev, "fmoe_route_experts_backward", ctypes.byref(r),
+          grad_w.data_ptr(), logits.data_ptr(), topk_idx.data_ptr(), out.data_ptr())
     return out
 
 

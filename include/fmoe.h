@@ -418,6 +418,50 @@ int fmoe_fp4_dequantize(const fmoe_fp4_matrix* q, void* out, int32_t dtype, void
 int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* b, void* out, int32_t dtype,
                     void* stream);
 
+/* The expert layer on 4-bit weights: fmoe_forward_routed (kernel.cu:1006-1199 and :864-891 on
+ * FP8 weights) with hidden states quantised by the layer and both products in 4 bits.
+ *   x     = the hidden rows, quantised with input_scale
+ *   h     = (x W13[:I]^T) * silu(x W13[I:]^T), quantised with intermediate_scale
+ *   out_t = sum_k w_k h W2^T over the picks of the local experts, the rows rounded to bf16
+ *           before they are summed in fp32
+ * Picks outside [local_expert_offset, local_expert_offset + num_local_experts) take no part;
+ * an expert may be named twice. */
+typedef struct fmoe_fp4_problem {
+  int64_t num_tokens;
+  int32_t hidden_size;         /* a multiple of 32, <= 16384 */
+  int32_t intermediate_size;   /* a multiple of 32, <= 16384 */
+  int32_t num_local_experts;   /* <= 256 */
+  int32_t top_k;               /* <= 32 */
+  int32_t local_expert_offset;
+  int32_t format;              /* fmoe_fp4_format of the weights and the activations */
+  int32_t dtype;               /* fmoe_dtype of hidden_states */
+} fmoe_fp4_problem;
+
+/* Device pointers, contiguous, 16-byte aligned; weights laid out as fmoe_fp4_matrix says.
+ * The global scales (nvfp4 only) are NULL for 1. */
+typedef struct fmoe_fp4_tensors {
+  const void* hidden_states;  /* [T, H] */
+  const int32_t* topk_idx;    /* [T, top_k] expert ids, -1 for none */
+  const float* topk_w;        /* [T, top_k] */
+  const void* w13;            /* codes of [E_local, 2I, H] (rows [0,I) gate, [I,2I) up) */
+  const void* w13_scales;
+  const float* w13_global;    /* [E_local] or NULL */
+  const void* w2;             /* codes of [E_local, H, I] */
+  const void* w2_scales;
+  const float* w2_global;
+  const float* input_scale;         /* [1] or NULL */
+  const float* intermediate_scale;  /* [1] or NULL */
+  void* output;               /* [T, H] bf16, written completely */
+} fmoe_fp4_tensors;
+
+/* Scratch bytes of fmoe_fp4_forward. */
+int fmoe_fp4_workspace_size(const fmoe_fp4_problem* p, size_t* bytes);
+
+/* One call at a time per workspace (256-byte aligned). Asynchronous on `stream`; can be
+ * captured into a graph. */
+int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensors* t, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
