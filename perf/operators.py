@@ -21,9 +21,8 @@ _BLOCK = {"mxfp4": 32, "nvfp4": 16}  # values that share one scale
 
 
 def _fmoe():
-    path = str(Path(__file__).resolve().parent.parent / "fused-moe-yws_b200")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if "fmoe_b200" not in sys.modules:  # once: a program imports the package before its first step
+        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "fused-moe-yws_b200"))
     import fmoe_b200
 
     return fmoe_b200
