@@ -66,12 +66,25 @@ struct Cfg {
   static_assert(kStageBytes % 1024 == 0, "stage alignment");
 };
 
+// True for one lane of a fully active warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // scale tile (128 rows x 4 blocks) -> 4 tensor memory columns: lane l, column j holds the four
 // scale bytes of row 32 j + l
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-  const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3FFF)  // start address
-                        | ((uint64_t)8 << 16) | ((uint64_t)8 << 32)  // 8-row groups 128 B apart
-                        | ((uint64_t)1 << 46);             // descriptor version; no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF)            // start address
+         | ((uint64_t)8 << 16) | ((uint64_t)8 << 32)  // 8-row groups 128 B apart
+         | ((uint64_t)1 << 46);                       // descriptor version; no swizzle
+}
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
                : "memory");
 }
@@ -107,6 +120,28 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, int half) {
          | ((uint32_t)(n >> 3) << 17)                        // N / 8
          | (kFormat == FMOE_MXFP4 ? 1u << 23 : 0u)           // scales are e8m0 (else e4m3)
          | (1u << 27);                                       // M / 128
+}
+
+// The scale copies and MMAs of a K step (kMmas of K = 64) on one stage. Scale tiles are 512
+// bytes: 32 in descriptor units.
+template <int kFormat, int BN, int kMmas>
+__device__ __forceinline__ void issue_step(uint32_t d, uint64_t ad, uint64_t bd, uint64_t sd,
+                                           uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  using C = Cfg<kFormat, BN>;
+  constexpr int kPer = kFormat == FMOE_MXFP4 ? 2 : 1;  // MMAs per scale tile
+#pragma unroll
+  for (int j = 0; j < (kMmas + kPer - 1) / kPer; ++j) {
+    copy_scales(sfa + 4 * j, sd + 32 * j);
+#pragma unroll
+    for (int r = 0; r < C::kRuns; ++r)
+      copy_scales(sfb + 4 * (j * C::kRuns + r), sd + (1 + r) * (C::kRunBytes / 16) + 32 * j);
+  }
+#pragma unroll
+  for (int q = 0; q < kMmas; ++q) {
+    const int j = q / kPer;
+    mma_fp4<kFormat>(d, ad + 2 * q, bd + 2 * q, idesc_fp4<kFormat>(BN, q % kPer * 2), sfa + 4 * j,
+                     sfb + 4 * j * C::kRuns, q > 0 ? 1u : accumulate);
+  }
 }
 
 struct Tile {
@@ -317,59 +352,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ------------------------------------------------------------------ MMAs
-      int it = 0, n = 0;
-      bool ok = true;
-      Tile t;
-      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
-        if (n >= kBack &&
-            !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag)) {
+    // -------------------------------------------------------------------- MMAs
+    // The whole warp runs this loop and one elected lane issues: the operands stay in uniform
+    // registers.
+    int it = 0, n = 0;
+    bool ok = true;
+    Tile t;
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t st0 = __shfl_sync(0xffffffffu, smem_addr(stages), 0);
+    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
+      if (n >= kBack &&
+          !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag))
+        ok = false;
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = base + (n & 1) * C::kAcc1;
+      for (int k = 0; k < steps; ++k, ++it) {
+        const int s = it % S;
+        // the scale slot's last reader, two steps back
+        if ((it >= 2 && !mbar_wait(&empty[(it - 2) % S], ((it - 2) / S) & 1, abort_flag)) ||
+            !mbar_wait(&full[s], (it / S) & 1, abort_flag))
+          ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + (n & 1) * C::kAcc1;
-        for (int k = 0; k < steps; ++k, ++it) {
-          const int s = it % S;
-          // the scale slot's last reader, two steps back
-          if ((it >= 2 && !mbar_wait(&empty[(it - 2) % S], ((it - 2) / S) & 1, abort_flag)) ||
-              !mbar_wait(&full[s], (it / S) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t st = smem_addr(stages + s * C::kStageBytes);
-          const uint32_t sc = st + kABytes + C::kBBytes;
-          const uint32_t sfa = tmem + C::kScales + (it & 1) * C::kSlotCols;
-          const uint32_t sfb = sfa + C::kSfaCols;
-          const uint64_t ad = smem_desc_kmajor(st, 128);
-          const uint64_t bd = smem_desc_kmajor(st + kABytes, 128);
-          const int tiles = min(C::kScaleTiles, across - k * C::kScaleTiles);
-          for (int j = 0; j < tiles; ++j) {
-            copy_scales(sfa + 4 * j, sc + j * kTileBytes);
-#pragma unroll
-            for (int r = 0; r < C::kRuns; ++r)
-              copy_scales(sfb + 4 * (j * C::kRuns + r),
-                          sc + (1 + r) * C::kRunBytes + j * kTileBytes);
-          }
-          const int mmas = min(4, (p.K - k * kStepCols + 63) / 64);
-          for (int q = 0; q < mmas; ++q) {
-            const int j = kFormat == FMOE_MXFP4 ? q / 2 : q;
-            const int half = kFormat == FMOE_MXFP4 ? (q & 1) * 2 : 0;
-            mma_fp4<kFormat>(d, ad + 2 * q, bd + 2 * q, idesc_fp4<kFormat>(BN, half), sfa + 4 * j,
-                             sfb + 4 * j * C::kRuns, (k | q) != 0);
-          }
+        const uint32_t st = st0 + s * C::kStageBytes;
+        const uint32_t sfa = base + C::kScales + (it & 1) * C::kSlotCols;
+        const uint32_t sfb = sfa + C::kSfaCols;
+        const uint64_t ad = smem_desc_kmajor(st, 128);
+        const uint64_t bd = smem_desc_kmajor(st + kABytes, 128);
+        const uint64_t sd = scale_desc(st + kABytes + C::kBBytes);
+        const int mmas = min(4, (p.K - k * kStepCols + 63) / 64);
+        if (elect_one()) {
+          if (mmas == 4) issue_step<kFormat, BN, 4>(d, ad, bd, sd, sfa, sfb, k != 0);
+          else if (mmas == 3) issue_step<kFormat, BN, 3>(d, ad, bd, sd, sfa, sfb, k != 0);
+          else if (mmas == 2) issue_step<kFormat, BN, 2>(d, ad, bd, sd, sfa, sfb, k != 0);
+          else issue_step<kFormat, BN, 1>(d, ad, bd, sd, sfa, sfb, k != 0);
           tc_commit(&empty[s]);
+          if (k == steps - 1) tc_commit(&tfull[n & 1]);
         }
-        if (ok) tc_commit(&tfull[n & 1]);
+        __syncwarp();
       }
-      if (!ok) {
-        atomicOr(err, kErrTimeoutMma);
-        *abort_flag = 1;
-      }
-      // all issued MMAs must retire before tensor memory is released
-      static const int zero = 0;
+    }
+    if (!ok && lane == 0) {
+      atomicOr(err, kErrTimeoutMma);
+      *abort_flag = 1;
+    }
+    // all issued MMAs must retire before tensor memory is released
+    static const int zero = 0;
+    if (elect_one()) {
       tc_commit(mma_done);
       mbar_wait(mma_done, 0, &zero);
     }
