@@ -94,79 +94,172 @@ __device__ __forceinline__ V warp_sum(V v) {
 
 // exp(x - top) with the top itself at exactly 1, also where it is +inf (which then shares
 // the whole mass with the other infinities, the limit of the softmax).
-__device__ __forceinline__ double exp_below(float x, float top) {
-  return x == top ? 1.0 : exp((double)x - (double)top);
-}
-__device__ __forceinline__ float exp_below_f(float x, float top) {
+__device__ __forceinline__ float exp_below(float x, float top) {
   return x == top ? 1.0f : expf(x - top);
 }
+__device__ __forceinline__ double exp_below(double x, double top) {
+  return x == top ? 1.0 : exp(x - top);
+}
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-// Picks the token's experts: lane k returns the k-th one, or -1.
-template <int EPL>
-__device__ __forceinline__ int select_experts(const RouterArgs& a, const float (&x)[EPL],
-                                              int lane) {
+// Order-preserving map of a float to an unsigned key; 0 is below every number.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 ranks with 0
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// The best of the lanes' (value, expert) pairs, the lowest expert on a tie; INT_MAX: none.
+__device__ __forceinline__ void warp_best(float& v, int& e) {
+  const uint32_t key = e == INT_MAX ? 0u : key_of(v);
+  const uint32_t top = __reduce_max_sync(kAll, key);
+  e = (int)__reduce_min_sync(kAll, key == top ? (uint32_t)e : (uint32_t)INT_MAX);
+  v = __uint_as_float((top & 0x80000000u) ? (top & 0x7fffffffu) : ~top);
+}
+__device__ __forceinline__ void warp_best(double& v, int& e) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const double pv = __shfl_xor_sync(kAll, v, o);
+    const int pe = __shfl_xor_sync(kAll, e, o);
+    if (pe != INT_MAX && (e == INT_MAX || pv > v || (pv == v && pe < e))) {
+      v = pv;
+      e = pe;
+    }
+  }
+}
+
+// Picks the token's experts: lane k gets the k-th one, or -1. V = float: false where the scores
+// do not tell the order (the picks are then void). A score's error in single precision:
+//   softmax  the exponential 2^-22 and its argument's rounding (together below 2^-22 of the
+//            row's largest score), the sum and the division: (EPL + 16) 2^-24 of the largest
+//   sigmoid  exponential, sum, division: 8 * 2^-24
+// and the bias adds 2^-24 of the sum. Two scores further apart than twice that have the order
+// they seem to have. V = double decides the rest; it resolves 2^-52. Without a bias the picks
+// follow the logits, which need no arithmetic.
+template <int EPL, typename V>
+__device__ __forceinline__ bool select_experts(const RouterArgs& a, const float (&x)[EPL],
+                                               int lane, int& pick) {
+  constexpr bool kFast = sizeof(V) == 4;
+  const V kNone = (V)neg_inf();
   const int e0 = lane * EPL;
-  double worth[EPL], c[EPL];
-  if (a.softmax) {
+  const bool by_group = a.n_group > 1;
+  const bool scored = a.bias || (by_group && !a.group_max);
+  V worth[EPL], c[EPL];
+  float tol = 0.0f;  // twice the error of a score
+  if (!scored) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) worth[j] = (V)x[j];
+  } else if (a.softmax) {
     float top = neg_inf();
 #pragma unroll
     for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
     top = warp_max(top);
-    double sum = 0.0;
+    V sum = (V)0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      worth[j] = x[j] > neg_inf() ? exp_below(x[j], top) : 0.0;
+      worth[j] = x[j] > neg_inf() ? exp_below((V)x[j], (V)top) : (V)0;
       sum += worth[j];
     }
     sum = warp_sum(sum);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) worth[j] = sum > 0.0 ? worth[j] / sum : 0.0;
+    for (int j = 0; j < EPL; ++j) worth[j] = sum > (V)0 ? worth[j] / sum : (V)0;
+    if (kFast) tol = (EPL + 16) * 0x1p-23f / fmaxf((float)sum, 1.0f);
   } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) worth[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+    for (int j = 0; j < EPL; ++j) worth[j] = (V)1 / ((V)1 + exp_of(-(V)x[j]));
+    if (kFast) tol = 8 * 0x1p-23f;
   }
   uint32_t live = 0;
+  if (a.bias) {
+    float far = 0.0f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (e0 + j >= a.E) continue;
+      const float b = load_bias(a, e0 + j);
+      worth[j] += (V)b;
+      if (kFast && b > neg_inf()) far = fmaxf(far, fabsf(b));
+    }
+    if (kFast) tol += (1.0f + warp_max(far)) * 0x1p-23f;
+  }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
-    if (a.bias && e0 + j < a.E) worth[j] += (double)load_bias(a, e0 + j);
-    c[j] = a.bias ? worth[j] : (double)x[j];
-    if (x[j] > neg_inf() && c[j] > (double)neg_inf()) live |= 1u << j;
+    c[j] = a.bias ? worth[j] : (V)x[j];
+    if (x[j] > neg_inf() && c[j] > kNone) live |= 1u << j;
   }
-  if (a.n_group > 1) {
+  bool sure = true;
+  if (by_group) {
     const int G = a.E / a.n_group;
-    double mine = (double)neg_inf();  // lane g: the score of group g
-    for (int g = 0; g < a.n_group; ++g) {
-      double m1 = (double)neg_inf(), m2 = (double)neg_inf();
+    V mine = kNone;  // the score of the lane's group: lane g's, or lane / span's
+    int own = lane, span = 1;
+    // groups of whole lanes: the lanes of a group merge their two best
+    const bool whole = EPL * 32 == a.E && 32 % a.n_group == 0;
+    if (whole) {
+      span = 32 / a.n_group;
+      own = lane / span;
+      V m1 = kNone, m2 = kNone;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        const int e = e0 + j;
-        if (((live >> j) & 1u) && e >= g * G && e < g * G + G) {
-          const double v = a.group_max ? c[j] : worth[j];
-          m2 = fmax(m2, fmin(m1, v));
-          m1 = fmax(m1, v);
+      for (int j = 0; j < EPL; ++j)
+        if ((live >> j) & 1u) {
+          const V v = a.group_max ? c[j] : worth[j];
+          m2 = v > m1 ? m1 : (v > m2 ? v : m2);
+          m1 = v > m1 ? v : m1;
         }
+      for (int o = 1; o < span; o <<= 1) {
+        const V p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
+        const V low = m1 < p1 ? m1 : p1, second = m2 > p2 ? m2 : p2;
+        m1 = m1 < p1 ? p1 : m1;
+        m2 = low > second ? low : second;
       }
+      mine = a.group_max ? m1 : m1 + m2;
+    } else {
+      for (int g = 0; g < a.n_group; ++g) {
+        V m1 = kNone, m2 = kNone;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        const double p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
-        m2 = fmax(fmin(m1, p1), fmax(m2, p2));
-        m1 = fmax(m1, p1);
+        for (int j = 0; j < EPL; ++j) {
+          const int e = e0 + j;
+          if (((live >> j) & 1u) && e >= g * G && e < g * G + G) {
+            const V v = a.group_max ? c[j] : worth[j];
+            m2 = v > m1 ? m1 : (v > m2 ? v : m2);
+            m1 = v > m1 ? v : m1;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const V p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
+          const V low = m1 < p1 ? m1 : p1, second = m2 > p2 ? m2 : p2;
+          m1 = m1 < p1 ? p1 : m1;
+          m2 = low > second ? low : second;
+        }
+        if (lane == g) mine = a.group_max ? m1 : m1 + m2;
       }
-      if (lane == g) mine = a.group_max ? m1 : m1 + m2;
     }
     int rank = 0;
     for (int h = 0; h < a.n_group; ++h) {
-      const double v = __shfl_sync(kAll, mine, h);
-      rank += v > mine || (v == mine && h < lane);
+      const V v = __shfl_sync(kAll, mine, h * span);
+      rank += v > mine || (v == mine && h < own);
     }
-    const uint32_t kept = __ballot_sync(kAll, lane < a.n_group && rank < a.topk_group);
+    const uint32_t votes = __ballot_sync(kAll, own < a.n_group && rank < a.topk_group);
+    if (kFast && scored) {
+      // a kept and a dropped group whose scores are not told apart
+      for (int h = 0; h < a.n_group; ++h) {
+        const V v = __shfl_sync(kAll, mine, h * span);
+        const bool other = ((votes >> (h * span)) & 1u) != ((votes >> lane) & 1u);
+        if (own < a.n_group && other && !(fabsf((float)(v - mine)) > 2.0f * tol)) sure = false;
+      }
+    }
+    if (whole) {
+      if (!((votes >> lane) & 1u)) live = 0;
+    } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (e0 + j < a.E && !((kept >> ((e0 + j) / G)) & 1u)) live &= ~(1u << j);
+      for (int j = 0; j < EPL; ++j)
+        if (e0 + j < a.E && !((votes >> ((e0 + j) / G)) & 1u)) live &= ~(1u << j);
+    }
   }
-  int pick = -1;
-  for (int k = 0; k < a.K; ++k) {
-    double best = (double)neg_inf();
+  pick = -1;
+  const bool compare = kFast && a.bias != nullptr;
+  V last = (V)0;
+  for (int k = 0; k < a.K + (compare ? 1 : 0); ++k) {
+    V best = kNone;
     int at = INT_MAX;
 #pragma unroll
     for (int j = 0; j < EPL; ++j)
@@ -174,20 +267,15 @@ __device__ __forceinline__ int select_experts(const RouterArgs& a, const float (
         best = c[j];
         at = e0 + j;
       }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const double pv = __shfl_xor_sync(kAll, best, o);
-      const int pe = __shfl_xor_sync(kAll, at, o);
-      if (pv > best || (pv == best && pe < at)) {
-        best = pv;
-        at = pe;
-      }
-    }
+    warp_best(best, at);
     if (at == INT_MAX) break;  // fewer usable experts than top_k
+    if (compare && k > 0 && !((float)(last - best) > tol)) sure = false;
+    last = best;
+    if (k == a.K) break;
     if (at / EPL == lane) live &= ~(1u << (at % EPL));
     if (lane == k) pick = at;
   }
-  return pick;
+  return !kFast || __all_sync(kAll, sure);
 }
 
 // The weights of the picked experts (lane k < K holds pick k) from their logits. For plain
@@ -197,11 +285,11 @@ __device__ __forceinline__ float pick_weight(const RouterArgs& a, int pick, floa
   if (a.softmax) {
     if (a.renorm) {
       const float m = warp_max(pick >= 0 ? x : neg_inf());
-      const float e = pick >= 0 ? exp_below_f(x, m) : 0.0f;
+      const float e = pick >= 0 ? exp_below(x, m) : 0.0f;
       const float total = warp_sum(e);
       return pick >= 0 ? e / total : 0.0f;
     }
-    return pick >= 0 ? exp_below_f(x, top) / sum : 0.0f;
+    return pick >= 0 ? exp_below(x, top) / sum : 0.0f;
   }
   return pick >= 0 ? 1.0f / (1.0f + expf(-x)) : 0.0f;
 }
@@ -214,7 +302,7 @@ __device__ __forceinline__ void row_softmax(const float (&x)[EPL], float& top, f
   top = warp_max(top);
   sum = 0.0f;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) sum += x[j] > neg_inf() ? exp_below_f(x[j], top) : 0.0f;
+  for (int j = 0; j < EPL; ++j) sum += x[j] > neg_inf() ? exp_below(x[j], top) : 0.0f;
   sum = warp_sum(sum);
 }
 
@@ -225,7 +313,8 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_kernel(Router
   if (t >= a.T) return;
   float x[EPL];
   load_logits<EPL, In>(a, t, lane, x);
-  const int pick = select_experts<EPL>(a, x, lane);
+  int pick;
+  if (!select_experts<EPL, float>(a, x, lane, pick)) select_experts<EPL, double>(a, x, lane, pick);
   float top = 0.0f, sum = 1.0f;
   if (a.softmax && !a.renorm) row_softmax<EPL>(x, top, sum);
   const float xp =
@@ -290,7 +379,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(R
   float dx[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j)
-    dx[j] = dense && x[j] > neg_inf() ? -all * (exp_below_f(x[j], top) / sum) : 0.0f;
+    dx[j] = dense && x[j] > neg_inf() ? -all * (exp_below(x[j], top) / sum) : 0.0f;
   for (int k = 0; k < a.K; ++k) {
     const int at = __shfl_sync(kAll, pick, k) - e0;
     const float dk = __shfl_sync(kAll, d, k);
