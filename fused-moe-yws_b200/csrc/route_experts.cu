@@ -18,6 +18,7 @@
 
 #include <climits>
 #include <string>
+#include <type_traits>
 
 #include "fmoe.h"
 #include "fmoe_common.cuh"
@@ -39,6 +40,8 @@ struct RouterArgs {
   int E, K, n_group, topk_group;
   bool softmax, group_max, renorm;
   float scale;
+  bool wide;         // rows, bias and gradient rows allow a lane's values to move as vectors
+  bool by_key;       // select_by_key takes these groups
   int* idx;          // [T, K]
   float* w;          // [T, K]
   // backward
@@ -62,15 +65,64 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
+// N consecutive elements, as vectors of up to 16 bytes where `wide` says they are aligned and
+// inside the row.
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, bool wide, int inside, T (&v)[N]) {
+  constexpr int kBytes = N * (int)sizeof(T);
+  if constexpr (kBytes >= 4) {
+    if (wide) {
+      if constexpr (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i)
+          reinterpret_cast<uint4*>(v)[i] =
+              inside > 0 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+      } else if constexpr (kBytes == 8) {
+        *reinterpret_cast<uint2*>(v) =
+            inside > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+      } else {
+        *reinterpret_cast<uint32_t*>(v) = inside > 0 ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = j < inside ? p[j] : T();
+}
+
+template <int N, typename T>
+__device__ __forceinline__ void store_n(T* p, bool wide, int inside, const T (&v)[N]) {
+  constexpr int kBytes = N * (int)sizeof(T);
+  if constexpr (kBytes >= 4) {
+    if (wide) {
+      if (inside <= 0) return;
+      if constexpr (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i)
+          reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+      } else if constexpr (kBytes == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+      } else {
+        *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(v);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < inside) p[j] = v[j];
+}
+
 // The lane's logits; experts past E and unusable ones (NaN) become -inf.
 template <int EPL, typename In>
 __device__ __forceinline__ void load_logits(const RouterArgs& a, int64_t t, int lane,
                                             float (&x)[EPL]) {
-  const In* row = static_cast<const In*>(a.logits) + t * a.stride;
   const int e0 = lane * EPL;
+  alignas(16) In raw[EPL];
+  load_n(static_cast<const In*>(a.logits) + t * a.stride + e0, a.wide, a.E - e0, raw);
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
-    const float v = e0 + j < a.E ? to_float(row[e0 + j]) : neg_inf();
+    const float v = e0 + j < a.E ? to_float(raw[j]) : neg_inf();
     x[j] = v > neg_inf() ? v : neg_inf();
   }
 }
@@ -126,6 +178,178 @@ __device__ __forceinline__ void warp_best(double& v, int& e) {
       e = pe;
     }
   }
+}
+
+template <int EPL>
+__device__ __forceinline__ void load_bias_n(const RouterArgs& a, int lane, float (&b)[EPL]) {
+  const int e0 = lane * EPL;
+  if (a.bias_bf16) {
+    alignas(16) __nv_bfloat16 raw[EPL];
+    load_n(static_cast<const __nv_bfloat16*>(a.bias) + e0, a.wide, a.E - e0, raw);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) b[j] = __bfloat162float(raw[j]);
+  } else {
+    alignas(16) float raw[EPL];
+    load_n(static_cast<const float*>(a.bias) + e0, a.wide, a.E - e0, raw);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) b[j] = raw[j];
+  }
+}
+
+// Descending sort of a lane's keys (odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&p)[N]) {
+#pragma unroll
+  for (int q = 1; q < N; q <<= 1)
+#pragma unroll
+    for (int k = q; k >= 1; k >>= 1)
+#pragma unroll
+      for (int j = k % q; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * q) == (i + j + k) / (2 * q)) {
+            const uint32_t lo = min(p[i + j], p[i + j + k]);
+            p[i + j] = max(p[i + j], p[i + j + k]);
+            p[i + j + k] = lo;
+          }
+}
+
+// Picks by one 32-bit key an expert: its value in the high bits, its index (reversed, so that
+// the lower index wins a tie) in the low ones. A lane sorts its keys once; a round is one warp
+// maximum and a shift in the winning lane, a quarter of the instructions of comparing (value,
+// index) pairs (16384 x 256 on B200: 40 -> 15 us).
+//   bias     the score on a grid over the row's range, 24 bits for up to 256 experts; false
+//            where two scores that matter are not told apart (see select_experts: tol is twice
+//            a score's error, the grid adds 5 steps for two roundings and a product)
+//   no bias  16-bit logits as they are: exact
+// Groups are whole runs of lanes, or there are none.
+template <int EPL, typename In>
+__device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (&x)[EPL], int lane,
+                                              int& pick) {
+  constexpr int kIndexBits = EPL == 1 ? 5 : EPL == 2 ? 6 : EPL == 4 ? 7 : EPL == 8 ? 8
+                             : EPL == 16 ? 9 : 10;
+  const int e0 = lane * EPL;
+  uint32_t p[EPL];
+  int bits = 16;
+  uint32_t near = 0;  // keys whose values differ by no more are not told apart
+  if (a.bias) {
+    bits = kIndexBits;
+    float c[EPL], b[EPL];
+    load_bias_n<EPL>(a, lane, b);
+    float tol;
+    if (a.softmax) {
+      float top = neg_inf();
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
+      top = warp_max(top);
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        c[j] = x[j] > neg_inf() ? exp_below(x[j], top) : 0.0f;
+        sum += c[j];
+      }
+      sum = warp_sum(sum);
+      const float by = 1.0f / fmaxf(sum, 1.0f);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c[j] *= by;
+      tol = (EPL + 16) * 0x1p-23f * by;
+    } else {
+      // the fast exponential and division: 2^-22 and |x| 2^-23 of e^-x; times the slope of
+      // 1 / (1 + e^-x), at most 1/4 (with |x|: 0.23), and 2^-22 for the division
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c[j] = __fdividef(1.0f, 1.0f + __expf(-x[j]));
+      tol = 16 * 0x1p-23f;
+    }
+    float low = __int_as_float(0x7f800000), high = neg_inf();
+    bool live[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      c[j] += b[j];
+      live[j] = x[j] > neg_inf() && c[j] > neg_inf();
+      if (live[j]) {
+        low = fminf(low, c[j]);
+        high = fmaxf(high, c[j]);
+      }
+    }
+    low = -warp_max(-low);
+    high = warp_max(high);
+    if (!(high >= low)) {  // no expert at all
+      pick = -1;
+      return true;
+    }
+    tol += fmaxf(fabsf(low), fabsf(high)) * 0x1p-23f;
+    const float range = high - low;
+    // 24 bits are what a float resolves; the margin takes the roundings above the top
+    constexpr int kGrid = 32 - kIndexBits < 24 ? 32 - kIndexBits : 24;
+    const float step = (float)((1 << kGrid) - 64) / range;
+    if (!(range > tol) || !(step < 0x1p60f)) return false;  // infinite, or nothing told apart
+    near = (uint32_t)fminf(tol * step, 0x1p30f) + 5;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const uint32_t v = (uint32_t)((c[j] - low) * step) + 1;
+      p[j] = live[j] ? (v << kIndexBits) | ((1u << kIndexBits) - 1 - (e0 + j)) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      uint32_t v;
+      if constexpr (sizeof(In) == 2 && !std::is_same<In, __half>::value) {
+        v = key_of(x[j]) >> 16;
+      } else {
+        const uint32_t h = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
+        v = ((h & 0x8000u) ? ~h : h | 0x8000u) & 0xffffu;
+      }
+      p[j] = x[j] > neg_inf() ? (v << 16) | (0xffffu - (e0 + j)) : 0u;
+    }
+  }
+  sort_keys(p);
+  bool sure = true;
+  if (a.n_group > 1) {
+    const int span = 32 / a.n_group, own = lane / span;
+    uint32_t m1 = p[0] >> bits, m2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] >> bits : 0u;
+    for (int o = 1; o < span; o <<= 1) {
+      const uint32_t p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
+      m2 = max(min(m1, p1), max(m2, p2));
+      m1 = max(m1, p1);
+    }
+    // a group with too few usable experts is below all others (-1) and tells apart by its index
+    const int mine = a.group_max ? (m1 ? (int)m1 : -1) : (m2 ? (int)(m1 + m2) : -1);
+    int rank = 0;
+    for (int h = 0; h < a.n_group; ++h) {
+      const int v = __shfl_sync(kAll, mine, h * span);
+      rank += v > mine || (v == mine && h < own);
+    }
+    const bool keep = rank < a.topk_group;
+    if (near) {
+      const uint32_t votes = __ballot_sync(kAll, keep);
+      for (int h = 0; h < a.n_group; ++h) {
+        const int v = __shfl_sync(kAll, mine, h * span);
+        if ((bool)((votes >> (h * span)) & 1u) != keep && v >= 0 && mine >= 0 &&
+            (uint32_t)abs(v - mine) <= 2 * near)
+          sure = false;
+      }
+    }
+    if (!keep) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) p[j] = 0u;
+    }
+  }
+  pick = -1;
+  uint32_t last = 0;
+  const uint32_t mask = (1u << bits) - 1;
+  for (int k = 0; k < a.K + (near ? 1 : 0); ++k) {
+    const uint32_t top = __reduce_max_sync(kAll, p[0]);
+    if (top == 0) break;  // fewer usable experts than top_k
+    if (near && k > 0 && last - (top >> bits) <= near) sure = false;
+    last = top >> bits;
+    if (lane == k && k < a.K) pick = (int)(mask - (top & mask));
+    if (p[0] == top) {
+#pragma unroll
+      for (int j = 0; j + 1 < EPL; ++j) p[j] = p[j + 1];
+      p[EPL - 1] = 0u;
+    }
+  }
+  return __all_sync(kAll, sure);
 }
 
 // Picks the token's experts: lane k gets the k-th one, or -1. V = float: false where the scores
@@ -314,7 +538,10 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_kernel(Router
   float x[EPL];
   load_logits<EPL, In>(a, t, lane, x);
   int pick;
-  if (!select_experts<EPL, float>(a, x, lane, pick)) select_experts<EPL, double>(a, x, lane, pick);
+  bool sure = false;
+  if (a.by_key && (a.bias || sizeof(In) == 2)) sure = select_by_key<EPL, In>(a, x, lane, pick);
+  else sure = select_experts<EPL, float>(a, x, lane, pick);
+  if (!sure) select_experts<EPL, double>(a, x, lane, pick);
   float top = 0.0f, sum = 1.0f;
   if (a.softmax && !a.renorm) row_softmax<EPL>(x, top, sum);
   const float xp =
@@ -387,9 +614,10 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(R
     for (int j = 0; j < EPL; ++j)
       if (at == j) dx[j] += dk;
   }
+  alignas(16) In raw[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j)
-    if (e0 + j < a.E) out[e0 + j] = from_float<In>(dx[j]);
+  for (int j = 0; j < EPL; ++j) raw[j] = from_float<In>(dx[j]);
+  store_n(out + e0, a.wide, a.E - e0, raw);
 }
 
 // ------------------------------------------------------------------------------ host side
@@ -445,8 +673,23 @@ RouterArgs router_args(const fmoe_router* r, const void* logits) {
   return a;
 }
 
+// Whether a lane's N values of every row, of the bias and of a gradient row are aligned vectors
+// that lie inside the row or outside of it.
+template <int N, typename In>
+bool vectors(const RouterArgs& a) {
+  const size_t bytes = N * sizeof(In) < 16 ? N * sizeof(In) : 16;
+  const size_t bias = a.bias_bf16 ? 2 : 4;
+  const size_t bias_bytes = N * bias < 16 ? N * bias : 16;
+  return a.E % N == 0 && a.stride % N == 0 && bytes >= 4 && bias_bytes >= 4 &&
+         reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
+         reinterpret_cast<uintptr_t>(a.grad_logits) % bytes == 0 &&
+         reinterpret_cast<uintptr_t>(a.bias) % bias_bytes == 0;
+}
+
 template <int EPL, typename In>
-void launch_router(const RouterArgs& a, bool backward, cudaStream_t stream) {
+void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
+  a.wide = vectors<EPL, In>(a);
+  a.by_key = a.n_group == 1 || (EPL * 32 == a.E && 32 % a.n_group == 0 && (a.bias || a.group_max));
   const unsigned grid = (unsigned)((a.T + kRouterWarps - 1) / kRouterWarps);
   if (backward)
     route_experts_grad_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
