@@ -132,10 +132,16 @@ __device__ __forceinline__ float load_bias(const RouterArgs& a, int e) {
                      : static_cast<const float*>(a.bias)[e];
 }
 
+// The warp's largest and smallest value in one instruction; NaN takes no part.
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
-  return v;
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_min(float v) {
+  float r;
+  asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 template <typename V>
 __device__ __forceinline__ V warp_sum(V v) {
@@ -169,15 +175,17 @@ __device__ __forceinline__ void warp_best(float& v, int& e) {
   v = __uint_as_float((top & 0x80000000u) ? (top & 0x7fffffffu) : ~top);
 }
 __device__ __forceinline__ void warp_best(double& v, int& e) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double pv = __shfl_xor_sync(kAll, v, o);
-    const int pe = __shfl_xor_sync(kAll, e, o);
-    if (pe != INT_MAX && (e == INT_MAX || pv > v || (pv == v && pe < e))) {
-      v = pv;
-      e = pe;
-    }
+  unsigned long long key = 0;  // the order of the doubles, in two halves for the reductions
+  if (e != INT_MAX) {
+    const long long b = __double_as_longlong(v + 0.0);
+    key = b < 0 ? ~(unsigned long long)b : (unsigned long long)b | (1ull << 63);
   }
+  const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
+  const uint32_t top_hi = __reduce_max_sync(kAll, hi);
+  const uint32_t top_lo = __reduce_max_sync(kAll, hi == top_hi ? lo : 0u);
+  e = (int)__reduce_min_sync(kAll, hi == top_hi && lo == top_lo ? (uint32_t)e : (uint32_t)INT_MAX);
+  const unsigned long long top = (unsigned long long)top_hi << 32 | top_lo;
+  v = __longlong_as_double((long long)(top >> 63 ? top & ~(1ull << 63) : ~top));
 }
 
 template <int EPL>
@@ -214,90 +222,111 @@ __device__ __forceinline__ void sort_keys(uint32_t (&p)[N]) {
           }
 }
 
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Picks by one 32-bit key an expert: its value in the high bits, its index (reversed, so that
 // the lower index wins a tie) in the low ones. A lane sorts its keys once; a round is one warp
-// maximum and a shift in the winning lane, a quarter of the instructions of comparing (value,
-// index) pairs (16384 x 256 on B200: 40 -> 15 us).
-//   bias     the score on a grid over the row's range, 24 bits for up to 256 experts; false
+// maximum and a shift in the winning lane.
+//   bias     the score on a grid over the row's range, 23 bits for up to 512 experts; false
 //            where two scores that matter are not told apart (see select_experts: tol is twice
-//            a score's error, the grid adds 5 steps for two roundings and a product)
+//            a score's error, the grid adds two steps for its roundings)
 //   no bias  16-bit logits as they are: exact
-// Groups are whole runs of lanes, or there are none.
+// Groups are whole runs of lanes, or there are none. Issue-bound: 1150 instructions a token
+// with compared (value, index) pairs, 28 us for 16384 x 256 on B200.
 template <int EPL, typename In>
 __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (&x)[EPL], int lane,
                                               int& pick) {
-  constexpr int kIndexBits = EPL == 1 ? 5 : EPL == 2 ? 6 : EPL == 4 ? 7 : EPL == 8 ? 8
-                             : EPL == 16 ? 9 : 10;
+  constexpr int kScoreBits = EPL <= 8 ? 8 : EPL == 16 ? 9 : 10;  // index bits beside a score
   const int e0 = lane * EPL;
   uint32_t p[EPL];
-  int bits = 16;
-  uint32_t near = 0;  // keys whose values differ by no more are not told apart
+  const int bits = a.bias ? kScoreBits : 16;
+  uint32_t near = 0;  // values that differ by no more are not told apart
   if (a.bias) {
-    bits = kIndexBits;
+    const float kNaN = __int_as_float(0x7fffffff), kLog2e = 1.4426950408889634f;
     float c[EPL], b[EPL];
     load_bias_n<EPL>(a, lane, b);
     float tol;
+    // experts that may not be used become NaN, which minima and maxima pass over
     if (a.softmax) {
       float top = neg_inf();
 #pragma unroll
       for (int j = 0; j < EPL; ++j) top = fmaxf(top, x[j]);
       top = warp_max(top);
+      if (!(fabsf(top) < 1e30f)) return false;  // an infinity, or no expert at all
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
-        c[j] = x[j] > neg_inf() ? exp_below(x[j], top) : 0.0f;
+        c[j] = fast_exp2((x[j] - top) * kLog2e);
         sum += c[j];
       }
       sum = warp_sum(sum);
-      const float by = 1.0f / fmaxf(sum, 1.0f);
+      const float by = fast_reciprocal(sum);
 #pragma unroll
       for (int j = 0; j < EPL; ++j) c[j] *= by;
       tol = (EPL + 16) * 0x1p-23f * by;
     } else {
-      // the fast exponential and division: 2^-22 and |x| 2^-23 of e^-x; times the slope of
-      // 1 / (1 + e^-x), at most 1/4 (with |x|: 0.23), and 2^-22 for the division
+      // e^-x is off by 2^-22 and |x| 2^-23, times the slope of 1 / (1 + e^-x), at most 1/4 (with
+      // |x|: 0.23); the reciprocal by 2^-23
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) c[j] = __fdividef(1.0f, 1.0f + __expf(-x[j]));
-      tol = 16 * 0x1p-23f;
+      for (int j = 0; j < EPL; ++j) c[j] = fast_reciprocal(1.0f + fast_exp2(x[j] * -kLog2e));
+      tol = 8 * 0x1p-23f;
     }
     float low = __int_as_float(0x7f800000), high = neg_inf();
-    bool live[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      c[j] += b[j];
-      live[j] = x[j] > neg_inf() && c[j] > neg_inf();
-      if (live[j]) {
-        low = fminf(low, c[j]);
-        high = fmaxf(high, c[j]);
-      }
+      c[j] = x[j] > neg_inf() ? c[j] + b[j] : kNaN;
+      low = fminf(low, c[j]);
+      high = fmaxf(high, c[j]);
     }
-    low = -warp_max(-low);
+    low = warp_min(low);
+    if (low == neg_inf()) {  // experts that the bias takes out
+      low = __int_as_float(0x7f800000);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        c[j] = c[j] > neg_inf() ? c[j] : kNaN;
+        low = fminf(low, c[j]);
+      }
+      low = warp_min(low);
+    }
     high = warp_max(high);
-    if (!(high >= low)) {  // no expert at all
+    if (!(high >= low) || high == neg_inf()) {  // no expert at all
       pick = -1;
       return true;
     }
     tol += fmaxf(fabsf(low), fabsf(high)) * 0x1p-23f;
+    // Grid steps are the low mantissa bits of 2^23 + 16 + (c - low) step: one multiply-add
+    // (its offset's rounding is the same for every expert) and no conversion.
+    constexpr int kGrid = 32 - kScoreBits < 23 ? 32 - kScoreBits : 23;
     const float range = high - low;
-    // 24 bits are what a float resolves; the margin takes the roundings above the top
-    constexpr int kGrid = 32 - kIndexBits < 24 ? 32 - kIndexBits : 24;
     const float step = (float)((1 << kGrid) - 64) / range;
     if (!(range > tol) || !(step < 0x1p60f)) return false;  // infinite, or nothing told apart
-    near = (uint32_t)fminf(tol * step, 0x1p30f) + 5;
+    const float offset = __fmaf_rn(-low, step, 0x1p23f + 16.0f);
+    if (!(fabsf(offset) < 0x1p25f)) return false;  // a range far from zero: too coarse a sum
+    near = (uint32_t)(tol * step) + 4;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      const uint32_t v = (uint32_t)((c[j] - low) * step) + 1;
-      p[j] = live[j] ? (v << kIndexBits) | ((1u << kIndexBits) - 1 - (e0 + j)) : 0u;
+      const uint32_t v = __float_as_uint(__fmaf_rn(c[j], step, offset));
+      // the shift drops the exponent
+      p[j] = c[j] == c[j] ? (v << kScoreBits) | ((1u << kScoreBits) - 1 - (e0 + j)) : 0u;
     }
   } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       uint32_t v;
-      if constexpr (sizeof(In) == 2 && !std::is_same<In, __half>::value) {
-        v = key_of(x[j]) >> 16;
-      } else {
+      if constexpr (std::is_same<In, __half>::value) {
         const uint32_t h = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
         v = ((h & 0x8000u) ? ~h : h | 0x8000u) & 0xffffu;
+      } else {
+        v = key_of(x[j]) >> 16;
       }
       p[j] = x[j] > neg_inf() ? (v << 16) | (0xffffu - (e0 + j)) : 0u;
     }
@@ -312,22 +341,21 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (
       m2 = max(min(m1, p1), max(m2, p2));
       m1 = max(m1, p1);
     }
-    // a group with too few usable experts is below all others (-1) and tells apart by its index
-    const int mine = a.group_max ? (m1 ? (int)m1 : -1) : (m2 ? (int)(m1 + m2) : -1);
+    // 0: too few usable experts, below all others; such groups are told apart by their index
+    const uint32_t mine = a.group_max ? m1 : m2 ? m1 + m2 : 0u;
+    // a group's lanes share the comparisons with the other groups
     int rank = 0;
-    for (int h = 0; h < a.n_group; ++h) {
-      const int v = __shfl_sync(kAll, mine, h * span);
-      rank += v > mine || (v == mine && h < own);
+    for (int i = 0; i < a.n_group; i += span) {
+      const int h = i + lane % span;  // past the last group where there are few
+      const uint32_t v = __shfl_sync(kAll, mine, h * span & 31);
+      rank += h < a.n_group && (v > mine || (v == mine && h < own));
     }
+    for (int o = 1; o < span; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
     const bool keep = rank < a.topk_group;
     if (near) {
-      const uint32_t votes = __ballot_sync(kAll, keep);
-      for (int h = 0; h < a.n_group; ++h) {
-        const int v = __shfl_sync(kAll, mine, h * span);
-        if ((bool)((votes >> (h * span)) & 1u) != keep && v >= 0 && mine >= 0 &&
-            (uint32_t)abs(v - mine) <= 2 * near)
-          sure = false;
-      }
+      const uint32_t worst = __reduce_min_sync(kAll, keep ? mine : 0xffffffffu);
+      const uint32_t best = __reduce_max_sync(kAll, keep ? 0u : mine);
+      if (best > 0 && worst - best <= 2 * near) sure = false;
     }
     if (!keep) {
 #pragma unroll
@@ -335,21 +363,24 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (
     }
   }
   pick = -1;
-  uint32_t last = 0;
   const uint32_t mask = (1u << bits) - 1;
-  for (int k = 0; k < a.K + (near ? 1 : 0); ++k) {
+  uint32_t gap = 0xffffffffu, last = 0;  // smallest distance of neighbours in the order
+  const int rounds = a.K + (near ? 1 : 0);
+  for (int k = 0; k < rounds; ++k) {
     const uint32_t top = __reduce_max_sync(kAll, p[0]);
     if (top == 0) break;  // fewer usable experts than top_k
-    if (near && k > 0 && last - (top >> bits) <= near) sure = false;
-    last = top >> bits;
-    if (lane == k && k < a.K) pick = (int)(mask - (top & mask));
+    if (k > 0) gap = min(gap, last - top);
+    last = top;
+    if (lane == k) pick = (int)(mask - (top & mask));
     if (p[0] == top) {
 #pragma unroll
       for (int j = 0; j + 1 < EPL; ++j) p[j] = p[j + 1];
       p[EPL - 1] = 0u;
     }
   }
-  return __all_sync(kAll, sure);
+  if (lane >= a.K) pick = -1;
+  if (near && (gap >> bits) <= near) sure = false;
+  return sure;
 }
 
 // Picks the token's experts: lane k gets the k-th one, or -1. V = float: false where the scores
@@ -602,22 +633,27 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(R
   }
   if (pick < 0) d = 0.0f;
   const float all = dense ? warp_sum(d) : 0.0f;
+  // every expert's dense part as vectors, then the picks' places again with their own
   const int e0 = lane * EPL;
-  float dx[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j)
-    dx[j] = dense && x[j] > neg_inf() ? -all * (exp_below(x[j], top) / sum) : 0.0f;
-  for (int k = 0; k < a.K; ++k) {
-    const int at = __shfl_sync(kAll, pick, k) - e0;
-    const float dk = __shfl_sync(kAll, d, k);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (at == j) dx[j] += dk;
-  }
   alignas(16) In raw[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) raw[j] = from_float<In>(dx[j]);
+  for (int j = 0; j < EPL; ++j)
+    raw[j] = from_float<In>(
+        dense && x[j] > neg_inf() ? -all * (exp_below(x[j], top) / sum) : 0.0f);
   store_n(out + e0, a.wide, a.E - e0, raw);
+  const unsigned same = __match_any_sync(kAll, pick);
+  if (__any_sync(kAll, pick >= 0 && __popc(same) > 1)) {
+    // an expert named several times: its first pick takes the terms of all
+    float total = 0.0f;
+    for (int k = 0; k < a.K; ++k) {
+      const float dk = __shfl_sync(kAll, d, k);
+      if ((same >> k) & 1u) total += dk;
+    }
+    d = total;
+    if (lane != __ffs(same) - 1) pick = -1;
+  }
+  __syncwarp();  // the row's vectors are stored
+  if (pick >= 0) out[pick] = from_float<In>(dense ? d - all * s : d);
 }
 
 // ------------------------------------------------------------------------------ host side

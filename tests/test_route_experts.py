@@ -48,6 +48,8 @@ RULES = [
     (256, 8, 8, 4, "top2"), (256, 8, 8, 4, "max"), (60, 4, 1, 1, "top2"), (60, 6, 4, 2, "top2"),
     (1, 1, 1, 1, "top2"), (8, 2, 1, 1, "max"), (16, 4, 4, 2, "top2"), (72, 8, 3, 1, "max"),
     (160, 6, 8, 3, "max"), (512, 16, 32, 7, "top2"), (1000, 32, 4, 2, "top2"), (33, 32, 1, 1, "max"),
+    (64, 6, 2, 1, "top2"), (128, 8, 4, 2, "max"), (32, 4, 16, 5, "max"), (512, 8, 2, 1, "max"),
+    (1024, 8, 4, 3, "top2"),
 ]
 
 
