@@ -103,11 +103,73 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t top, float& multiply) {
   multiply = __int_as_float((int)((254 - byte) << 23));
   return top >= 0x7f800000u ? 255u : byte;
 }
-__device__ __forceinline__ uint32_t nv_scale(uint32_t top, float global, float& divide) {
-  const uint32_t byte =
-      e4m3_byte(fminf(__fdiv_rn(__int_as_float((int)top), __fmul_rn(6.0f, global)), 448.0f));
-  divide = __fmul_rn(e4m3_value(byte), global);
+// The correctly rounded quotient x / d from the rounded reciprocal r of d by one residual step,
+// q = x r, q + (x - q d) r (Markstein 1990), where these stay finite.
+__device__ __forceinline__ float quotient(float x, float d, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q, d, x), r, q);
+}
+__device__ __forceinline__ bool tame(float d) { return d > 0x1p-100f && d < 0x1p100f; }
+
+// The divisor 6 g of a block's largest magnitude, and its reciprocal: once per matrix.
+struct NvDivisor {
+  float global, six, r;
+};
+__device__ __forceinline__ NvDivisor nv_divisor(float global) {
+  const float six = __fmul_rn(6.0f, global);
+  return {global, six, __frcp_rn(six)};
+}
+__device__ __forceinline__ uint32_t nv_scale(uint32_t top, const NvDivisor& n, float& divide) {
+  const float t = __int_as_float((int)top);
+  const float s = tame(n.six) && t < 0x1p20f ? quotient(t, n.six, n.r) : __fdiv_rn(t, n.six);
+  const uint32_t byte = e4m3_byte(fminf(s, 448.0f));
+  divide = __fmul_rn(e4m3_value(byte), n.global);
   return top >= 0x7f800000u ? 127u : byte;
+}
+
+// Encodes 16 values (an nvfp4 block, or half an mxfp4 block whose largest magnitude both halves
+// know): the codes of v[0..7] and v[8..15] and the block's scale byte. The quotients are the
+// correctly rounded ones of the definition.
+template <int kFormat>
+__device__ __forceinline__ uint32_t encode16(float (&v)[16], uint32_t top, const NvDivisor& n,
+                                             uint32_t& lo, uint32_t& hi) {
+  uint32_t byte;
+  float by;
+  if constexpr (kFormat == FMOE_MXFP4) {
+    byte = mx_scale(top, by);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(v[i], by);
+  } else {
+    byte = nv_scale(top, n, by);
+    const float r = __frcp_rn(by);
+    if (tame(by) && __int_as_float((int)top) * r < 0x1p20f) {
+      // two at a time: each half of a packed operation rounds like the single one
+      const float2 r2 = make_float2(r, r), d2 = make_float2(-by, -by);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float2 x = make_float2(v[i], v[i + 1]);
+        const float2 q = __fmul2_rn(x, r2);
+        const float2 y = __ffma2_rn(__ffma2_rn(q, d2, x), r2, q);
+        v[i] = y.x;
+        v[i + 1] = y.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = by > 0.0f ? __fdiv_rn(v[i], by) : __fmul_rn(v[i], 0.0f);
+    }
+  }
+  const float a[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+  const float b[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+  lo = encode8(a);
+  hi = encode8(b);
+  return byte;
+}
+
+// gate * silu(up) with the fast exponential and division: a few units in the last place, far
+// below the 4 bits that it is rounded to
+__device__ __forceinline__ float swiglu(float gate, float up) {
+  return gate * __fdividef(up, 1.0f + __expf(-up));
 }
 
 }  // namespace fp4

@@ -1,9 +1,10 @@
 // fp4_quant.cu -- quantisation of a matrix to 4-bit blocks, and back.
 //
-// A CTA takes 128 rows x 256 columns: the 2 KB (nvfp4) or 1 KB (mxfp4) of scales of that
-// square lie back to back (fp4.cuh), so they are gathered in shared memory and leave in whole
-// lines. A thread takes 16 consecutive values of a row: one nvfp4 block, or half an mxfp4
-// block, whose other half its neighbour holds.
+// Bound by memory: 2 to 4 bytes a value in, 4.5 bits out (and back). A CTA takes 128 rows x 128
+// columns: the 1 KB (nvfp4) or 512 bytes (mxfp4) of scales of that square lie back to back
+// (fp4.cuh), so they are gathered in shared memory and leave in whole lines. A thread takes 16
+// consecutive values of a row: one nvfp4 block, or half an mxfp4 block, whose other half its
+// neighbour holds; four rows' loads are in flight together.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -21,8 +22,10 @@ namespace {
 
 using namespace fp4;
 
-constexpr int kCols = 256;      // columns per CTA
-constexpr int kThreads = 256;   // 16 rows at a time, 16 threads a row
+constexpr int kCols = 128;             // columns per CTA
+constexpr int kThreads = 256;
+constexpr int kAcross = kCols / 16;    // threads a row
+constexpr int kDown = kThreads / kAcross;
 
 template <typename T>
 __device__ __forceinline__ float as_float(T v);
@@ -45,31 +48,59 @@ __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half as_type<__half>(float v) { return __float2half_rn(v); }
 
-// 16 consecutive elements, by 16-byte loads where the address allows them.
+// 16 consecutive elements as they lie in memory, by 16-byte loads where the address allows them.
+template <typename T>
+struct Raw {
+  uint32_t w[4 * sizeof(T)];
+};
 template <typename T, bool kWide>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
+__device__ __forceinline__ Raw<T> load16(const T* p) {
+  Raw<T> r;
   if constexpr (kWide) {
-    constexpr int kPer = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-      uint4 raw = *reinterpret_cast<const uint4*>(p + i * kPer);
-      const T* e = reinterpret_cast<const T*>(&raw);
+    for (int i = 0; i < (int)sizeof(T); ++i)
+      reinterpret_cast<uint4*>(r.w)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) v[i * kPer + j] = as_float<T>(e[j]);
-    }
+    for (int i = 0; i < 16; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = as_float<T>(p[i]);
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      r.w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+    }
+  }
+  return r;
+}
+
+// The values, and the bits of the largest magnitude as fp32 (NaN above the infinity above the
+// numbers). 16-bit types are compared two at a time in their own bits, which order the same way.
+template <typename T>
+__device__ __forceinline__ uint32_t unpack16(const Raw<T>& r, float (&v)[16]) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = __uint_as_float(r.w[i]);
+      top = max(top, r.w[i] & 0x7fffffffu);
+    }
+    return top;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      top = __vmaxu2(top, r.w[i] & 0x7fff7fffu);
+      const T* e = reinterpret_cast<const T*>(&r.w[i]);
+      v[2 * i] = as_float<T>(e[0]);
+      v[2 * i + 1] = as_float<T>(e[1]);
+    }
+    const uint16_t most = (uint16_t)max(top & 0xffffu, top >> 16);
+    return __float_as_uint(as_float<T>(*reinterpret_cast<const T*>(&most))) & 0x7fffffffu;
   }
 }
 
-// gate * silu(up) with the fast exponential and division: a few units in the last place
-__device__ __forceinline__ float swiglu(float gate, float up) {
-  return gate * __fdividef(up, 1.0f + __expf(-up));
-}
-
 template <int kFormat, typename T, bool kWide, bool kSwiglu = false>
-__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(Fp4QuantArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fp4_quantize_kernel(Fp4QuantArgs a) {
   __shared__ __align__(16) uint8_t s_scale[kCols / tile_cols(kFormat) * kTileBytes];
   const int tid = threadIdx.x;
   const int64_t m0 = (int64_t)blockIdx.x * kTileRows;
@@ -80,54 +111,52 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(Fp4QuantArgs a) 
   const int across = tiles_across(a.cols, kFormat);
   const int first = c0 / tile_cols(kFormat);
   const int here = min(kCols / tile_cols(kFormat), across - first);
-  for (int i = tid; i < here * kTileBytes / 4; i += kThreads)
-    reinterpret_cast<uint32_t*>(s_scale)[i] = 0;
-  __syncthreads();
-  const float global = a.global ? a.global[a.global_step * e] : 1.0f;
+  const NvDivisor divisor = nv_divisor(a.global ? a.global[a.global_step * e] : 1.0f);
   const T* x = static_cast<const T*>(a.x) + e * a.batch_stride;
   uint8_t* codes = a.codes + (int64_t)e * a.rows * (a.cols / 2);
-  const int c = c0 + (tid & 15) * 16;
-  for (int r = tid >> 4; r < kTileRows; r += kThreads / 16) {
-    const int64_t m = m0 + r;
-    int64_t src = m;
-    if (m < a.rows && a.row_index) src = a.row_index[m];
-    // whole warps stay together: an mxfp4 block belongs to two lanes
-    const bool mine = m < a.rows && src >= 0 && c < a.cols;
-    float v[16] = {};
-    uint32_t top = 0;
-    if (mine) {
+  const int c = c0 + tid % kAcross * 16;
+  // kRows rows at a time, their loads in flight together. Whole warps stay together: an mxfp4
+  // block belongs to two lanes.
+  constexpr int kRows = kSwiglu ? 2 : 4;
+  for (int r0 = tid / kAcross; r0 < kTileRows; r0 += kRows * kDown) {
+    Raw<T> raw[kRows], second[kSwiglu ? kRows : 1];
+    bool mine[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int64_t m = m0 + r0 + u * kDown;
+      int64_t src = m;
+      if (m < a.rows && a.row_index) src = a.row_index[m];
+      mine[u] = m < a.rows && src >= 0 && c < a.cols;
+      if (kSwiglu) src = m;
+      raw[u] = {};
+      if (kSwiglu) second[kSwiglu ? u : 0] = {};
+      if (mine[u]) {
+        raw[u] = load16<T, kWide>(x + src * a.row_stride + c);
+        if constexpr (kSwiglu) second[u] = load16<T, kWide>(x + src * a.row_stride + a.cols + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int r = r0 + u * kDown;
+      float v[16];
+      uint32_t top = unpack16<T>(raw[u], v);
       if constexpr (kSwiglu) {
         float up[16];
-        load16<T, kWide>(x + m * a.row_stride + c, v);
-        load16<T, kWide>(x + m * a.row_stride + a.cols + c, up);
+        unpack16<T>(second[u], up);
+        top = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = swiglu(v[i], up[i]);
-      } else {
-        load16<T, kWide>(x + src * a.row_stride + c, v);
+        for (int i = 0; i < 16; ++i) {
+          v[i] = swiglu(v[i], up[i]);
+          top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
-    uint32_t byte;
-    if constexpr (kFormat == FMOE_MXFP4) {
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      float by;
-      byte = mx_scale(top, by);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(v[i], by);
-    } else {
-      float by;
-      byte = nv_scale(top, global, by);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = by > 0.0f ? __fdiv_rn(v[i], by) : __fmul_rn(v[i], 0.0f);
-    }
-    if (mine) {
-      const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-      const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
-      *reinterpret_cast<uint2*>(codes + m * (a.cols / 2) + c / 2) =
-          make_uint2(encode8(lo), encode8(hi));
+      if constexpr (kFormat == FMOE_MXFP4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      uint32_t lo, hi;
+      const uint32_t byte = encode16<kFormat>(v, top, divisor, lo, hi);
+      if (mine[u])
+        *reinterpret_cast<uint2*>(codes + (m0 + r) * (a.cols / 2) + c / 2) = make_uint2(lo, hi);
       const int block = (c - c0) / block_of(kFormat);
-      s_scale[block / 4 * kTileBytes + scale_offset(r, block)] = (uint8_t)byte;
+      s_scale[block / 4 * kTileBytes + scale_offset(r, block)] = mine[u] ? (uint8_t)byte : 0;
     }
   }
   __syncthreads();
@@ -154,17 +183,27 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(Fp4QuantArgs a
   const float global = a.global ? a.global[a.global_step * e] : 1.0f;
   const uint8_t* codes = a.codes + (int64_t)e * a.rows * (a.cols / 2);
   T* out = static_cast<T*>(a.out) + (int64_t)e * a.rows * a.cols;
-  const int c = c0 + (tid & 15) * 16;
+  const int c = c0 + tid % kAcross * 16;
   if (c >= a.cols) return;
-  for (int r = tid >> 4; r < kTileRows && m0 + r < a.rows; r += kThreads / 16) {
+  constexpr int kRows = kTileRows / kDown;
+  uint2 raw[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t m = m0 + tid / kAcross + u * kDown;
+    raw[u] = m < a.rows ? *reinterpret_cast<const uint2*>(codes + m * (a.cols / 2) + c / 2)
+                        : make_uint2(0, 0);
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int r = tid / kAcross + u * kDown;
     const int64_t m = m0 + r;
-    const uint2 raw = *reinterpret_cast<const uint2*>(codes + m * (a.cols / 2) + c / 2);
+    if (m >= a.rows) break;
     const int block = (c - c0) / block_of(kFormat);
     const float s = __fmul_rn(
         scale_value<kFormat>(s_scale[block / 4 * kTileBytes + scale_offset(r, block)]), global);
     float lo[8], hi[8];
-    decode8(raw.x, lo);
-    decode8(raw.y, hi);
+    decode8(raw[u].x, lo);
+    decode8(raw[u].y, hi);
     constexpr int kPer = 16 / (int)sizeof(T);
     uint4 packed[16 / kPer];
     T* t = reinterpret_cast<T*>(packed);
