@@ -13,6 +13,10 @@
 // MMAs of step k have retired. A scale operand starts at a whole scale tile (4 columns), so BN
 // is a multiple of 128.
 //
+// With swiglu, b holds gate and up rows: a tile takes 128 rows of each, and the epilogue turns the
+// two halves of its columns into the 4-bit blocks of gate * silu(up), so the fp32 product never
+// reaches memory.
+//
 // Tensor memory has 512 columns. At BN = 128 two accumulators lie side by side. At BN = 256
 // two of them and the scales do not fit: the accumulators overlap by 96 columns, which the
 // epilogue reads first, and the next tile starts as soon as those are in registers.
@@ -42,6 +46,8 @@ constexpr int kStepCols = 256;      // K values per step
 constexpr int kABytes = 128 * 128;
 constexpr int kSmemLimit = 232448;
 constexpr int kOverlap = 96;        // columns two 256-column accumulators share
+
+enum Epilogue { kStore, kSwiglu };
 
 template <int kFormat, int BN>
 struct Cfg {
@@ -147,7 +153,7 @@ __device__ __forceinline__ void issue_step(uint32_t d, uint64_t ad, uint64_t bd,
 struct Tile {
   int m;        // row tile of a
   int rows;     // rows present
-  int n0;       // first row of b
+  int n;        // column tile
   int e;        // matrix of b
 };
 
@@ -167,6 +173,10 @@ struct GemmFp4Args {
   const int* tile_first;
   const int* count;
   const float* row_w;
+  // swiglu: the 4-bit blocks of the N / 2 values a row
+  uint8_t* codes;
+  uint8_t* scales;
+  const float* gc;
   unsigned* sink;
 };
 
@@ -174,7 +184,7 @@ struct GemmFp4Args {
 // memory): an expert's tiles follow one another, its row tiles first, so that CTAs that run
 // together read the same rows of b.
 __device__ __forceinline__ bool tile_of(const GemmFp4Args& p, const int* first, const int* count,
-                                        int64_t i, int bn, Tile& t) {
+                                        int64_t i, Tile& t) {
   if (p.experts == 0) {
     if (i >= (int64_t)p.m_tiles * p.n_tiles) return false;
     const int64_t per = (int64_t)p.panel * p.n_tiles;
@@ -182,7 +192,7 @@ __device__ __forceinline__ bool tile_of(const GemmFp4Args& p, const int* first, 
     const int high = min(p.panel, p.m_tiles - m);
     const int r = (int)(i % per);
     t.m = m + r % high;
-    t.n0 = r / high * bn;
+    t.n = r / high;
     t.rows = (int)min((int64_t)128, p.M - (int64_t)t.m * 128);
     t.e = 0;
     return true;
@@ -199,7 +209,7 @@ __device__ __forceinline__ bool tile_of(const GemmFp4Args& p, const int* first, 
   const int j = (int)(i - (int64_t)first[low] * p.n_tiles);
   t.e = low;
   t.m = first[low] + j % tiles;
-  t.n0 = j / tiles * bn;
+  t.n = j / tiles;
   t.rows = min(128, count[low] - j % tiles * 128);
   return true;
 }
@@ -250,9 +260,37 @@ __device__ __forceinline__ void store32(const GemmFp4Args& p, int64_t m, int n,
   }
 }
 
-template <int kFormat, int BN>
+// Columns [col, col + 32) of a row's halves: gate * silu(up), as 4-bit blocks. Returns the scale
+// bytes, one (mxfp4) or two.
+template <int kFormat>
+__device__ __forceinline__ uint32_t swiglu32(const uint32_t (&gate)[32], const uint32_t (&up)[32],
+                                             float alpha, const NvDivisor& divisor, uint4& codes) {
+  float v[32];
+  uint32_t top[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    v[i] = swiglu(__uint_as_float(gate[i]) * alpha, __uint_as_float(up[i]) * alpha);
+    top[i / 16] = max(top[i / 16], __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  if (kFormat == FMOE_MXFP4) top[0] = top[1] = max(top[0], top[1]);
+  uint32_t bytes = 0;
+  uint32_t w[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = v[16 * h + i];
+    const uint32_t b = encode16<kFormat>(x, top[h], divisor, w[2 * h], w[2 * h + 1]);
+    bytes |= kFormat == FMOE_MXFP4 ? b : b << (8 * h);
+  }
+  codes = make_uint4(w[0], w[1], w[2], w[3]);
+  return bytes;
+}
+
+template <int kFormat, int BN, Epilogue kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_a32,
                     const __grid_constant__ CUtensorMap map_b, const GemmFp4Args p) {
   using C = Cfg<kFormat, BN>;
   __shared__ int s_first[kMaxExperts + 1], s_count[kMaxExperts];
@@ -285,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *err = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_a32);
     tma_prefetch_desc(&map_b);
   }
   if (warp == 1) {
@@ -317,9 +356,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       bool ok = true;
       Tile t;
-      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x) {
+      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x) {
         const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
-        const uint8_t* sb = p.sb + ((int64_t)t.e * tiles_down(p.N) + t.n0 / 128) * across * kTileBytes;
+        // the 128-row runs of b: next to each other, or gate and up rows
+        int row[C::kRuns], runs = 0;
+        const uint8_t* sb[C::kRuns];
+#pragma unroll
+        for (int r = 0; r < C::kRuns; ++r) {
+          row[r] = kEpi == kSwiglu ? t.n * 128 + r * (p.N / 2) : t.n * BN + r * 128;
+          if (row[r] < p.N) ++runs;  // a run past b's last row is not there
+          sb[r] = p.sb + ((int64_t)t.e * tiles_down(p.N) + row[r] / 128) * across * kTileBytes;
+        }
         for (int k = 0; k < steps; ++k, ++it) {
           const int s = it % S;
           if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
@@ -329,17 +376,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* st = stages + s * C::kStageBytes;
           uint8_t* sc = st + kABytes + C::kBBytes;
           const int have = min(C::kScaleTiles, across - k * C::kScaleTiles) * kTileBytes;
-          // runs of b past its last 128 rows do not exist
-          int runs = 1;
-          if constexpr (C::kRuns == 2) runs = t.n0 + 128 < p.N ? 2 : 1;
-          mbar_arrive_expect_tx(&full[s], kABytes + C::kBBytes + (1 + runs) * have);
-          tma_load_2d(st, &map_a, &full[s], k * 128, t.m * 128, keep);
-          tma_load_3d(st + kABytes, &map_b, &full[s], k * 128, t.n0, t.e, keep);
           const int64_t at = (int64_t)k * C::kScaleTiles * kTileBytes;
+          // few rows: boxes of 32 (the other rows of the stage keep what they held; a row of a
+          // only reaches its own row of the product)
+          const int boxes = t.rows > 64 ? 0 : (t.rows + 31) / 32;
+          mbar_arrive_expect_tx(&full[s], (boxes ? boxes * 4096 : kABytes) + have +
+                                              runs * (128 * 128 + have));
+#pragma unroll
+          for (int r = 0; r < C::kRuns; ++r) {
+            if (r >= runs) break;
+            tma_load_3d(st + kABytes + r * 128 * 128, &map_b, &full[s], k * 128, row[r], t.e, keep);
+            bulk_load_1d(sc + (1 + r) * C::kRunBytes, sb[r] + at, have, &full[s]);
+          }
+          if (boxes == 0) tma_load_2d(st, &map_a, &full[s], k * 128, t.m * 128, keep);
+          for (int x = 0; x < boxes; ++x)
+            tma_load_2d(st + x * 4096, &map_a32, &full[s], k * 128, t.m * 128 + 32 * x, keep);
           bulk_load_1d(sc, sa + at, have, &full[s]);
-          for (int r = 0; r < runs; ++r)
-            bulk_load_1d(sc + (1 + r) * C::kRunBytes,
-                         sb + (int64_t)r * across * kTileBytes + at, have, &full[s]);
         }
       }
       if (!ok) {
@@ -360,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Tile t;
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t st0 = __shfl_sync(0xffffffffu, smem_addr(stages), 0);
-    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
+    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x, ++n) {
       if (n >= kBack &&
           !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag))
         ok = false;
@@ -415,13 +467,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3;                   // tensor memory lanes 32 q .. 32 q + 31
     const int half = (warp - 2) >> 2;         // columns half * BN / 2 ..
     const float ga = p.ga ? *p.ga : 1.0f;
+    const NvDivisor divisor = nv_divisor(kEpi == kSwiglu && p.gc ? *p.gc : 1.0f);
     const bool wide = (int64_t)p.N * (p.dtype == FMOE_F32 ? 4 : 2) % 32 == 0 &&
                       reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
     constexpr int kChunks = BN / 64;          // 32-column chunks of this warp
     int n = 0;
     bool ok = true;
     Tile t;
-    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, BN, t); i += gridDim.x, ++n) {
+    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x, ++n) {
       if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
         ok = false;
         break;
@@ -432,7 +485,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t m = (int64_t)t.m * 128 + row;
       float alpha = p.gb ? ga * p.gb[t.e] : ga;
       if (p.row_w && row < t.rows) alpha *= p.row_w[m];
-      if constexpr (!C::kOverlapped) {
+      const int n0 = t.n * BN;
+      if constexpr (kEpi == kSwiglu) {
+        // this warp's 64 gate columns (col) and 64 up columns (128 + col). The side that lies in
+        // the columns shared with the next tile comes first: up in the first accumulator
+        // (160..255), gate in the second (0..95).
+        const bool first = (n & 1) == 0;
+        const uint32_t col = half * 64;
+        uint32_t s0[32], s1[32], o[32];
+        const uint32_t shared = acc + col + (first ? 128 : 0), other = acc + col + (first ? 0 : 128);
+        tmem_ld_32x32b<32>(shared, s0);
+        tmem_ld_32x32b<32>(shared + 32, s1);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[n & 1]);
+        const int I = p.N / 2, c0 = t.n * 128 + (int)col;
+        uint8_t* dst = p.codes + m * (I / 2) + c0 / 2;
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_ld_32x32b<32>(other + 32 * h, o);
+          tmem_ld_wait();
+          uint4 codes;
+          uint32_t b;
+          if (first) b = swiglu32<kFormat>(o, h ? s1 : s0, alpha, divisor, codes);
+          else b = swiglu32<kFormat>(h ? s1 : s0, o, alpha, divisor, codes);
+          bytes |= b << (kFormat == FMOE_MXFP4 ? 8 * h : 16 * h);
+          if (row < t.rows) *reinterpret_cast<uint4*>(dst + 16 * h) = codes;
+        }
+        if (row < t.rows) {
+          const int block = c0 / block_of(kFormat);
+          uint8_t* sc = p.scales +
+                        ((int64_t)t.m * tiles_across(I, kFormat) + block / 4) * kTileBytes +
+                        scale_offset(row, block);
+          if (kFormat == FMOE_MXFP4) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)bytes;
+          else *reinterpret_cast<uint32_t*>(sc) = bytes;
+        }
+      } else if constexpr (!C::kOverlapped) {
         const uint32_t col = half * (BN / 2);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
@@ -444,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[n & 1]);
           }
-          if (row < t.rows) store32(p, m, t.n0 + col + 32 * c, v, alpha, wide);
+          if (row < t.rows) store32(p, m, n0 + col + 32 * c, v, alpha, wide);
         }
       } else {
         // the columns that the next tile's accumulator shares with this one come first:
@@ -466,20 +556,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&tempty[n & 1]);
         if (shares) {
           if (row < t.rows) {
-            store32(p, m, t.n0 + c0, v0, alpha, wide);
-            store32(p, m, t.n0 + c0 + 32, v1, alpha, wide);
-            store32(p, m, t.n0 + c0 + 64, v2, alpha, wide);
+            store32(p, m, n0 + c0, v0, alpha, wide);
+            store32(p, m, n0 + c0 + 32, v1, alpha, wide);
+            store32(p, m, n0 + c0 + 64, v2, alpha, wide);
           }
           const uint32_t c1 = first ? col : col + 96;
           tmem_ld_32x32b<32>(acc + c1, v0);
           tmem_ld_wait();
-          if (row < t.rows) store32(p, m, t.n0 + c1, v0, alpha, wide);
+          if (row < t.rows) store32(p, m, n0 + c1, v0, alpha, wide);
         } else {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             tmem_ld_32x32b<32>(acc + col + 32 * c, v0);
             tmem_ld_wait();
-            if (row < t.rows) store32(p, m, t.n0 + col + 32 * c, v0, alpha, wide);
+            if (row < t.rows) store32(p, m, n0 + col + 32 * c, v0, alpha, wide);
           }
         }
       }
@@ -500,10 +590,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && *err != 0 && p.sink) report_device_error(p.sink, *err);
 }
 
-template <int kFormat, int BN>
-cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const GemmFp4Args& p, int grid,
-                   cudaStream_t stream) {
-  auto* fn = fp4_gemm_kernel<kFormat, BN>;
+struct Maps {
+  CUtensorMap a, a32, b;
+};
+
+template <int kFormat, int BN, Epilogue kEpi>
+cudaError_t launch(const Maps& maps, const GemmFp4Args& p, int grid, cudaStream_t stream) {
+  auto* fn = fp4_gemm_kernel<kFormat, BN, kEpi>;
   static thread_local int configured = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -515,14 +608,15 @@ cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const GemmFp4Args
     configured = dev;
   }
   return launch_pdl(fn, dim3((unsigned)grid), dim3(kThreads), Cfg<kFormat, BN>::kSmemBytes, stream,
-                    a, b, p);
+                    maps.a, maps.a32, maps.b, p);
 }
 
 template <int kFormat>
-cudaError_t launch(int bn, const CUtensorMap& a, const CUtensorMap& b, const GemmFp4Args& p,
-                   int grid, cudaStream_t stream) {
-  if (bn == 128) return launch<kFormat, 128>(a, b, p, grid, stream);
-  return launch<kFormat, 256>(a, b, p, grid, stream);
+cudaError_t launch(int bn, bool swiglu, const Maps& maps, const GemmFp4Args& p, int grid,
+                   cudaStream_t stream) {
+  if (swiglu) return launch<kFormat, 256, kSwiglu>(maps, p, grid, stream);
+  if (bn == 128) return launch<kFormat, 128, kStore>(maps, p, grid, stream);
+  return launch<kFormat, 256, kStore>(maps, p, grid, stream);
 }
 
 int bad(const std::string& msg) {
@@ -548,22 +642,28 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
   p.tile_first = g.tile_first;
   p.count = g.count;
   p.row_w = g.row_w;
+  p.codes = static_cast<uint8_t*>(g.codes);
+  p.scales = static_cast<uint8_t*>(g.scales);
+  p.gc = g.gc;
   p.m_tiles = (int)tiles_down(g.M);
   // the widest tile that still gives every SM one
+  const bool swiglu = g.codes != nullptr;
   int bn = 256;
-  while (bn > 128 && (int64_t)p.m_tiles * ((g.N + bn - 1) / bn) < sms) bn /= 2;
+  while (!swiglu && bn > 128 && (int64_t)p.m_tiles * ((g.N + bn - 1) / bn) < sms) bn /= 2;
   p.n_tiles = (g.N + bn - 1) / bn;
   p.panel = 8;
   p.sink = device_error_sink(stream);
-  CUtensorMap ma, mb;
-  int v = make_byte_map(&ma, g.a, g.K / 2, g.M, 0, 128, 128, "a");
+  Maps maps;
+  int v = make_byte_map(&maps.a, g.a, g.K / 2, g.M, 0, 128, 128, "a");
+  if (v == FMOE_OK) v = make_byte_map(&maps.a32, g.a, g.K / 2, g.M, 0, 128, 32, "a");
   if (v == FMOE_OK)
-    v = make_byte_map(&mb, g.b, g.K / 2, g.N, g.experts > 0 ? g.experts : 1, 128, bn, "b");
+    v = make_byte_map(&maps.b, g.b, g.K / 2, g.N, g.experts > 0 ? g.experts : 1, 128, 128, "b");
   if (v != FMOE_OK) return v;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   const int grid = (int)(tiles < sms ? tiles : sms);
-  const cudaError_t e = g.format == FMOE_MXFP4 ? launch<FMOE_MXFP4>(bn, ma, mb, p, grid, stream)
-                                               : launch<FMOE_NVFP4>(bn, ma, mb, p, grid, stream);
+  const cudaError_t e = g.format == FMOE_MXFP4
+                            ? launch<FMOE_MXFP4>(bn, swiglu, maps, p, grid, stream)
+                            : launch<FMOE_NVFP4>(bn, swiglu, maps, p, grid, stream);
   if (e == cudaSuccess) return FMOE_OK;
   set_last_error(std::string("4-bit product: ") + cudaGetErrorString(e));
   return FMOE_ERR_RUNTIME;

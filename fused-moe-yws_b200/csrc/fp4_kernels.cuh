@@ -50,6 +50,11 @@ struct Fp4Gemm {
   const int* tile_first;  // [experts + 1] on the device
   const int* count;       // [experts] on the device
   const float* row_w;     // or null: factor of each row of out
+  // Or, instead of out: b's rows are N / 2 gate and N / 2 up rows (N / 2 a multiple of 128), and
+  // gate * silu(up) goes to a 4-bit matrix [M, N / 2] with the global scale gc (null: 1).
+  void* codes;
+  void* scales;
+  const float* gc;
 };
 int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream);
 

@@ -3,7 +3,7 @@
 //   plan      (token, k) pairs of the local experts in expert order, stable; every expert's rows
 //             start at a multiple of 128, the row tile of the products
 //   quantise  the pairs' hidden rows, gathered, to 4-bit blocks
-//   product 1 with W13, then SwiGLU and quantisation to 4-bit blocks
+//   product 1 with W13, SwiGLU and quantisation to 4-bit blocks in its epilogue
 //   product 2 with W2, times the routing weight, to bf16 rows
 //   combine   a token's rows summed in the order of its picks (permute.cu)
 //
@@ -151,6 +151,10 @@ struct Layout {
       total;
 };
 
+// Gate and up rows start at whole scale tiles of W13: SwiGLU and quantisation run in the first
+// product's epilogue. Otherwise they are a pass of their own over an fp32 product.
+bool fused(const fmoe_fp4_problem* p) { return p->intermediate_size % 128 == 0; }
+
 Layout layout_of(const fmoe_fp4_problem* p) {
   Layout L = {};
   const int64_t pairs = p->num_tokens * p->top_k;
@@ -172,7 +176,7 @@ Layout layout_of(const fmoe_fp4_problem* p) {
   L.token_row = take((size_t)pairs * 4);
   L.xq = take(rows * (p->hidden_size / 2));
   L.xs = take(tiles * fp4::tiles_across(p->hidden_size, p->format) * fp4::kTileBytes);
-  L.hidden = take(rows * 2 * p->intermediate_size * 4);
+  L.hidden = take(fused(p) ? 0 : rows * 2 * p->intermediate_size * 4);
   L.cq = take(rows * (p->intermediate_size / 2));
   L.cs = take(tiles * fp4::tiles_across(p->intermediate_size, p->format) * fp4::kTileBytes);
   L.ow = take(rows * p->hidden_size * 2);
@@ -295,25 +299,34 @@ extern "C" int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensor
   g.K = H;
   g.ga = t->input_scale;
   g.gb = t->w13_global;
-  g.out = ws + L.hidden;
-  g.dtype = FMOE_F32;
   g.experts = E;
   g.tile_first = plan.tile_first;
   g.count = plan.count;
+  if (fused(p)) {
+    g.codes = ws + L.cq;
+    g.scales = ws + L.cs;
+    g.gc = t->intermediate_scale;
+  } else {
+    g.out = ws + L.hidden;
+    g.dtype = FMOE_F32;
+  }
   if ((v = launch_fp4_gemm(g, stream)) != FMOE_OK) return v;
 
-  q.x = ws + L.hidden;
-  q.row_stride = 2 * I;
-  q.cols = I;
-  q.global = t->intermediate_scale;
-  q.codes = ws + L.cq;
-  q.scales = ws + L.cs;
-  q.swiglu = true;
-  if ((e = launch_fp4_quantize(q, p->format, FMOE_F32, 1, stream)) != cudaSuccess)
-    return cuda_failed(e);
+  if (!fused(p)) {
+    q.x = ws + L.hidden;
+    q.row_stride = 2 * I;
+    q.cols = I;
+    q.global = t->intermediate_scale;
+    q.codes = ws + L.cq;
+    q.scales = ws + L.cs;
+    q.swiglu = true;
+    if ((e = launch_fp4_quantize(q, p->format, FMOE_F32, 1, stream)) != cudaSuccess)
+      return cuda_failed(e);
+  }
 
-  g.a = q.codes;
-  g.sa = q.scales;
+  g.codes = g.scales = nullptr;
+  g.a = ws + L.cq;
+  g.sa = ws + L.cs;
   g.b = t->w2;
   g.sb = t->w2_scales;
   g.N = H;
