@@ -70,20 +70,22 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_plan_rows_kernel(PlanArgs a)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   pdl_trigger();
-  for (int i = tid; i < kPlanWarps * kPlanExperts; i += kPlanThreads)
-    s_warp[i / kPlanExperts][i % kPlanExperts] = 0;
+  const int warps = blockDim.x / 32;  // a single CTA has as many as its pairs need
+  for (int w = warp; w < warps; w += warps)
+    for (int x = lane; x < a.experts; x += 32) s_warp[w][x] = 0;
   __syncthreads();
   const int64_t i = (int64_t)blockIdx.x * kPlanThreads + tid;
   const int e = local_expert(a, i);
+  const float weight = i < a.pairs ? a.w[i] : 0.0f;
   const unsigned same = __match_any_sync(0xffffffffu, e);
   const int rank = __popc(same & ((1u << lane) - 1u));
   if (e >= 0 && rank == 0) s_warp[warp][e] = __popc(same);
   __syncthreads();
-  if (tid < a.experts) {
+  for (int x = tid; x < a.experts; x += blockDim.x) {
     int run = 0;
-    for (int w = 0; w < kPlanWarps; ++w) {
-      const int n = s_warp[w][tid];
-      s_warp[w][tid] = run;
+    for (int w = 0; w < warps; ++w) {
+      const int n = s_warp[w][x];
+      s_warp[w][x] = run;
       run += n;
     }
     int total = run, before = 0;
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_plan_rows_kernel(PlanArgs a)
         int n[kBatch];
 #pragma unroll
         for (int q = 0; q < kBatch; ++q)
-          n[q] = c + q < (int)gridDim.x ? a.cta_count[(int64_t)(c + q) * a.experts + tid] : 0;
+          n[q] = c + q < (int)gridDim.x ? a.cta_count[(int64_t)(c + q) * a.experts + x] : 0;
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
           if (c + q < (int)blockIdx.x) before += n[q];
@@ -102,8 +104,8 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_plan_rows_kernel(PlanArgs a)
         }
       }
     }
-    s_total[tid] = total;
-    s_before[tid] = before;
+    s_total[x] = total;
+    s_before[x] = before;
   }
   __syncthreads();
   if (warp == 0) {
@@ -128,16 +130,16 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_plan_rows_kernel(PlanArgs a)
     if (e >= 0) {
       row = s_tile[e] * 128 + s_before[e] + s_warp[warp][e] + rank;
       a.row_token[row] = (int)(i / a.K);
-      a.row_w[row] = a.w[i];
+      a.row_w[row] = weight;
     }
     a.token_row[i] = row;
   }
   // the rows behind each expert's last
-  for (int x = blockIdx.x; x < a.experts; x += gridDim.x)
-    for (int r = s_tile[x] * 128 + s_total[x] + tid; r < s_tile[x + 1] * 128; r += kPlanThreads)
+  for (int x = blockIdx.x * warps + warp; x < a.experts; x += gridDim.x * warps)
+    for (int r = s_tile[x] * 128 + s_total[x] + lane; r < s_tile[x + 1] * 128; r += 32)
       a.row_token[r] = -1;
   if (blockIdx.x == 0) {
-    for (int x = tid; x <= a.experts; x += kPlanThreads) {
+    for (int x = tid; x <= a.experts; x += blockDim.x) {
       a.tile_first[x] = s_tile[x];
       if (x < a.experts) a.count[x] = s_total[x];
     }
@@ -271,8 +273,9 @@ extern "C" int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensor
     e = launch_pdl(fp4_plan_count_kernel, dim3((unsigned)L.ctas), dim3(kPlanThreads), 0, stream,
                    plan);
   if (e == cudaSuccess)
-    e = launch_pdl(fp4_plan_rows_kernel, dim3((unsigned)L.ctas), dim3(kPlanThreads), 0, stream,
-                   plan);
+    e = launch_pdl(fp4_plan_rows_kernel, dim3((unsigned)L.ctas),
+                   dim3(L.ctas > 1 ? kPlanThreads : (unsigned)((plan.pairs + 127) / 128 * 128)), 0,
+                   stream, plan);
   if (e != cudaSuccess) return cuda_failed(e);
 
   Fp4QuantArgs q = {};

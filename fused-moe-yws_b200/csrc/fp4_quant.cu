@@ -103,11 +103,9 @@ template <int kFormat, typename T, bool kWide, bool kSwiglu = false>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fp4_quantize_kernel(Fp4QuantArgs a) {
   __shared__ __align__(16) uint8_t s_scale[kCols / tile_cols(kFormat) * kTileBytes];
   const int tid = threadIdx.x;
-  const int64_t m0 = (int64_t)blockIdx.x * kTileRows;
   const int c0 = blockIdx.y * kCols, e = blockIdx.z;
   pdl_wait();
   pdl_trigger();
-  if (a.tiles_dev && (int)blockIdx.x >= *a.tiles_dev) return;  // row tiles nobody uses
   const int across = tiles_across(a.cols, kFormat);
   const int first = c0 / tile_cols(kFormat);
   const int here = min(kCols / tile_cols(kFormat), across - first);
@@ -115,55 +113,66 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fp4_quantize
   const T* x = static_cast<const T*>(a.x) + e * a.batch_stride;
   uint8_t* codes = a.codes + (int64_t)e * a.rows * (a.cols / 2);
   const int c = c0 + tid % kAcross * 16;
-  // kRows rows at a time, their loads in flight together. Whole warps stay together: an mxfp4
-  // block belongs to two lanes.
-  constexpr int kRows = kSwiglu ? 2 : 4;
-  for (int r0 = tid / kAcross; r0 < kTileRows; r0 += kRows * kDown) {
-    Raw<T> raw[kRows], second[kSwiglu ? kRows : 1];
-    bool mine[kRows];
+  // (a row tile each, but for gathered rows: there are fewer tiles than the buffers have room for)
+  const int tiles = a.tiles_dev ? *a.tiles_dev : (int)tiles_down(a.rows);
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t m0 = (int64_t)tile * kTileRows;
+    // kRows rows at a time, their loads in flight together. Whole warps stay together: an mxfp4
+    // block belongs to two lanes.
+    constexpr int kRows = kSwiglu ? 2 : 4;
+    for (int r0 = tid / kAcross; r0 < kTileRows; r0 += kRows * kDown) {
+      Raw<T> raw[kRows], second[kSwiglu ? kRows : 1];
+      bool mine[kRows];
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int64_t m = m0 + r0 + u * kDown;
-      int64_t src = m;
-      if (m < a.rows && a.row_index) src = a.row_index[m];
-      mine[u] = m < a.rows && src >= 0 && c < a.cols;
-      if (kSwiglu) src = m;
-      raw[u] = {};
-      if (kSwiglu) second[kSwiglu ? u : 0] = {};
-      if (mine[u]) {
-        raw[u] = load16<T, kWide>(x + src * a.row_stride + c);
-        if constexpr (kSwiglu) second[u] = load16<T, kWide>(x + src * a.row_stride + a.cols + c);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int r = r0 + u * kDown;
-      float v[16];
-      uint32_t top = unpack16<T>(raw[u], v);
-      if constexpr (kSwiglu) {
-        float up[16];
-        unpack16<T>(second[u], up);
-        top = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          v[i] = swiglu(v[i], up[i]);
-          top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      for (int u = 0; u < kRows; ++u) {
+        const int64_t m = m0 + r0 + u * kDown;
+        int64_t src = m;
+        if (m < a.rows && a.row_index) src = a.row_index[m];
+        mine[u] = m < a.rows && src >= 0 && c < a.cols;
+        if (kSwiglu) src = m;
+        raw[u] = {};
+        if (kSwiglu) second[kSwiglu ? u : 0] = {};
+        if (mine[u]) {
+          raw[u] = load16<T, kWide>(x + src * a.row_stride + c);
+          if constexpr (kSwiglu) second[u] = load16<T, kWide>(x + src * a.row_stride + a.cols + c);
         }
       }
-      if constexpr (kFormat == FMOE_MXFP4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      uint32_t lo, hi;
-      const uint32_t byte = encode16<kFormat>(v, top, divisor, lo, hi);
-      if (mine[u])
-        *reinterpret_cast<uint2*>(codes + (m0 + r) * (a.cols / 2) + c / 2) = make_uint2(lo, hi);
-      const int block = (c - c0) / block_of(kFormat);
-      s_scale[block / 4 * kTileBytes + scale_offset(r, block)] = mine[u] ? (uint8_t)byte : 0;
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int r = r0 + u * kDown;
+        const int block = (c - c0) / block_of(kFormat);
+        uint8_t* scale = s_scale + block / 4 * kTileBytes + scale_offset(r, block);
+        if (!__any_sync(0xffffffffu, mine[u])) {  // few rows a tile: most warps have none
+          *scale = 0;
+          continue;
+        }
+        float v[16];
+        uint32_t top = unpack16<T>(raw[u], v);
+        if constexpr (kSwiglu) {
+          float up[16];
+          unpack16<T>(second[u], up);
+          top = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = swiglu(v[i], up[i]);
+            top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+          }
+        }
+        if constexpr (kFormat == FMOE_MXFP4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        uint32_t lo, hi;
+        const uint32_t byte = encode16<kFormat>(v, top, divisor, lo, hi);
+        if (mine[u])
+          *reinterpret_cast<uint2*>(codes + (m0 + r) * (a.cols / 2) + c / 2) = make_uint2(lo, hi);
+        *scale = mine[u] ? (uint8_t)byte : 0;
+      }
     }
+    __syncthreads();
+    uint8_t* out = a.scales +
+                   (((int64_t)e * tiles_down(a.rows) + tile) * across + first) * kTileBytes;
+    for (int i = tid; i < here * kTileBytes / 16; i += kThreads)
+      reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s_scale)[i];
+    __syncthreads();
   }
-  __syncthreads();
-  uint8_t* out = a.scales +
-                 (((int64_t)e * tiles_down(a.rows) + blockIdx.x) * across + first) * kTileBytes;
-  for (int i = tid; i < here * kTileBytes / 16; i += kThreads)
-    reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s_scale)[i];
 }
 
 template <int kFormat, typename T>
@@ -219,8 +228,15 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(Fp4QuantArgs a
 }
 
 dim3 grid_of(const Fp4QuantArgs& a, int batch) {
-  return dim3((unsigned)tiles_down(a.rows), (unsigned)((a.cols + kCols - 1) / kCols),
-              (unsigned)batch);
+  const int across = (a.cols + kCols - 1) / kCols;
+  int64_t down = tiles_down(a.rows);
+  if (a.tiles_dev) {
+    // a few CTAs for every one that fits an SM: a grid over the whole capacity spent 18 of 40 us
+    // on CTAs without rows (4096 tokens, 32 of 256 experts)
+    const int64_t most = (24 * num_sms() + across - 1) / across;
+    down = down < most ? down : most;
+  }
+  return dim3((unsigned)down, (unsigned)across, (unsigned)batch);
 }
 
 template <int kFormat, typename T>

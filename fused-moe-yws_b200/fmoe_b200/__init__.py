@@ -182,8 +182,11 @@ def poll_device_error(device=None) -> int:
     bits = ctypes.c_int32(0)
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else device) \
         if not isinstance(device, torch.device) else device
-    with torch.cuda.device(dev):
+    if dev.index == torch.cuda.current_device():  # (entering a device context costs more than the poll)
         rc = lib.fmoe_poll_device_error(ctypes.byref(bits))
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.fmoe_poll_device_error(ctypes.byref(bits))
     if rc != FMOE_OK:
         _raise(lib, rc, "poll_device_error")
     return int(bits.value)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import functools
 
 import torch
 
@@ -193,12 +194,18 @@ def matmul_fp4(a: Fp4Tensor, b: Fp4Tensor, *, dtype: torch.dtype = torch.bfloat1
 
 
 def fp4_workspace_bytes(prob: FmoeFp4Problem) -> int:
+    """Scratch bytes of a forward_fp4 call with these sizes (fmoe_fp4_workspace_size)."""
     lib = load_library()
     n = ctypes.c_size_t(0)
     rc = lib.fmoe_fp4_workspace_size(ctypes.byref(prob), ctypes.byref(n))
     if rc != FMOE_OK:
         _raise(lib, rc, "fp4_workspace_bytes")
     return int(n.value)
+
+
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(*sizes):
+    return fp4_workspace_bytes(FmoeFp4Problem(*sizes))
 
 
 def forward_fp4(hidden_states: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
@@ -241,9 +248,9 @@ def forward_fp4(hidden_states: torch.Tensor, topk_idx: torch.Tensor, topk_w: tor
     scales = [None if g is None else _global_scale(g, [], dev, name, w13.format)
               for name, g in (("input_scale", input_scale),
                               ("intermediate_scale", intermediate_scale))]
-    prob = FmoeFp4Problem(T, H, I, E, K, int(local_expert_offset), m13.format,
-                          DTYPE_CODES[hidden_states.dtype])
-    nbytes = fp4_workspace_bytes(prob)
+    sizes = (T, H, I, E, K, int(local_expert_offset), m13.format, DTYPE_CODES[hidden_states.dtype])
+    prob = FmoeFp4Problem(*sizes)
+    nbytes = _workspace_bytes(*sizes)
     _raise_device_error(dev, "an earlier call on this device")
     out = _out(out, (T, H), torch.bfloat16, dev)
     if T == 0:
