@@ -44,22 +44,29 @@ constexpr int kThreads = 320;
 constexpr int kEpiWarps = 8;
 constexpr int kStepCols = 256;      // K values per step
 constexpr int kABytes = 128 * 128;
-constexpr int kSmemLimit = 232448;
+constexpr int kMaxExperts = 1024;   // of a grouped product; their row tiles and rows lie in
+constexpr int kStatic = (2 * kMaxExperts + 4) * 4;  // static shared memory
+constexpr int kSmemLimit = 232448 - kStatic;
 constexpr int kOverlap = 96;        // columns two 256-column accumulators share
 
 enum Epilogue { kStore, kSwiglu };
 
-template <int kFormat, int BN>
+// S > 1: a cluster of S CTAs takes a tile of at most 32 rows together, each a part of K (see
+// the kernel). The parts meet in `kExchange` bytes of shared memory: a slice of BN / S columns
+// from each other CTA.
+template <int kFormat, int BN, int S>
 struct Cfg {
+  static constexpr int kSlice = BN / S;                               // columns a CTA finishes
+  static constexpr int kExchange = (S - 1) * kSlice * 32 * 4;
   static constexpr int kScaleTiles = kStepCols / tile_cols(kFormat);  // per 128 rows and step
   static constexpr int kRunBytes = kScaleTiles * kTileBytes;
   static constexpr int kRuns = BN / 128;                              // 128-row runs of b
   static constexpr int kBBytes = BN * 128;
   static constexpr int kStageBytes = kABytes + kBBytes + (1 + kRuns) * kRunBytes;
   static constexpr int kFixed = 1024 + 512;
-  static constexpr int kStagesRaw = (kSmemLimit - kFixed) / kStageBytes;
+  static constexpr int kStagesRaw = (kSmemLimit - kFixed - kExchange) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
-  static constexpr int kSmemBytes = kFixed + kStages * kStageBytes;
+  static constexpr int kSmemBytes = kFixed + kExchange + kStages * kStageBytes;
   // tensor memory
   static constexpr bool kOverlapped = BN > 128;
   static constexpr int kAcc1 = kOverlapped ? BN - kOverlap : BN;      // second accumulator
@@ -130,10 +137,10 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, int half) {
 
 // The scale copies and MMAs of a K step (kMmas of K = 64) on one stage. Scale tiles are 512
 // bytes: 32 in descriptor units.
-template <int kFormat, int BN, int kMmas>
+template <int kFormat, int BN, int S, int kMmas>
 __device__ __forceinline__ void issue_step(uint32_t d, uint64_t ad, uint64_t bd, uint64_t sd,
                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  using C = Cfg<kFormat, BN>;
+  using C = Cfg<kFormat, BN, S>;
   constexpr int kPer = kFormat == FMOE_MXFP4 ? 2 : 1;  // MMAs per scale tile
 #pragma unroll
   for (int j = 0; j < (kMmas + kPer - 1) / kPer; ++j) {
@@ -156,8 +163,6 @@ struct Tile {
   int n;        // column tile
   int e;        // matrix of b
 };
-
-constexpr int kMaxExperts = 1024;
 
 struct GemmFp4Args {
   const uint8_t* sa;
@@ -309,18 +314,71 @@ __device__ __forceinline__ uint32_t swiglu32(const uint32_t (&gate)[32], const u
   return bytes;
 }
 
-template <int kFormat, int BN, Epilogue kEpi>
+// ---- the cluster's exchange -----------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of the same shared memory location in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                           uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void peer_arrive(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+// mbar_wait for a barrier that other CTAs of the cluster arrive on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
+                                                  const volatile int* abort) {
+  const uint32_t a = smem_addr(bar);
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort || globaltimer() - t0 > kWaitTimeoutNs) return false;
+  }
+}
+// All threads of all CTAs of the cluster.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\t"
+               "barrier.cluster.wait.acquire;" ::
+                   : "memory");
+}
+
+// kSplit > 1 (few rows, so fewer tiles than would keep every SM reading): in the last round of
+// tiles the CTAs of a cluster share a tile of at most 32 rows, each a part of the K steps. CTA r
+// finishes the tile's slice r of the columns (swiglu: of the features): the others store their
+// sums of that slice into its shared memory, it adds them in the order of the ranks. A tile of
+// more rows is the first CTA's, whole.
+template <int kFormat, int BN, Epilogue kEpi, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_a32,
                     const __grid_constant__ CUtensorMap map_b, const GemmFp4Args p) {
-  using C = Cfg<kFormat, BN>;
+  using C = Cfg<kFormat, BN, kSplit>;
   __shared__ int s_first[kMaxExperts + 1], s_count[kMaxExperts];
   constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stages + S * C::kStageBytes);
+  uint8_t* exchange = stages + S * C::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + C::kExchange);
   uint64_t* full = bars;         // [S] copies -> MMA
   uint64_t* empty = bars + 8;    // [S] MMA -> copies
   uint64_t* tfull = bars + 16;   // [2] MMA -> epilogue
@@ -329,6 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 22);
   int* err = reinterpret_cast<int*>(bars + 23);
+  uint64_t* xfull = bars + 24;   // the other CTAs' sums of this one's slice have come
+  uint64_t* xfree = bars + 25;   // the other CTAs have read this one's
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -341,6 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tempty[b], kEpiWarps);
     }
     mbar_init(mma_done, 1);
+    if (kSplit > 1) {
+      mbar_init(xfull, 32 * (kSplit - 1));
+      mbar_init(xfree, 32 * (kSplit - 1));
+    }
     *abort_flag = 0;
     *err = 0;
     fence_mbar_init();
@@ -353,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (kSplit > 1) cluster_sync();  // the peers' barriers are there
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -368,6 +433,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int steps = (p.K + kStepCols - 1) / kStepCols;
   const int across = tiles_across(p.K, kFormat);  // scale tiles per 128 rows
+  const uint32_t rank = kSplit > 1 ? cluster_rank() : 0;
+  // Tiles [0, whole) go round-robin to the CTAs, those behind them to the clusters: the last
+  // round where it would leave half of the CTAs without a tile.
+  const int64_t total = (int64_t)(p.experts ? s_first[p.experts] : p.m_tiles) * p.n_tiles;
+  const int64_t G = gridDim.x, clusters = G / kSplit;
+  int64_t whole = total;
+  if (kSplit > 1 && total % G <= clusters) whole = total - total % G;
+  const int64_t mine_whole = (whole - blockIdx.x + G - 1) / G;
+  // Tile j of this CTA and its K steps [k0, k1); false: no more. K steps none: not its part.
+  auto next = [&](int64_t j, Tile& t, int& k0, int& k1, bool& shared) {
+    k0 = 0;
+    k1 = steps;
+    shared = false;
+    if (j < mine_whole) return tile_of(p, s_first, s_count, blockIdx.x + j * G, t);
+    if (kSplit == 1) return false;
+    const int64_t i = whole + blockIdx.x / kSplit + (j - mine_whole) * clusters;
+    if (!tile_of(p, s_first, s_count, i, t)) return false;
+    shared = t.rows <= 32;
+    if (shared) {
+      k0 = steps * (int)rank / kSplit;
+      k1 = steps * ((int)rank + 1) / kSplit;
+    } else if (rank != 0) {
+      k1 = 0;
+    }
+    return true;
+  };
   // how many tiles back the accumulator of a tile must have been read
   constexpr int kBack = C::kOverlapped ? 1 : 2;
 
@@ -378,7 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       bool ok = true;
       Tile t;
-      for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x) {
+      int k0, k1;
+      bool shared;
+      for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
+        if (k1 == 0) continue;
         const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
         // the 128-row runs of b: next to each other, or gate and up rows
         int row[C::kRuns], runs = 0;
@@ -389,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (row[r] < p.N) ++runs;  // a run past b's last row is not there
           sb[r] = p.sb + ((int64_t)t.e * tiles_down(p.N) + row[r] / 128) * across * kTileBytes;
         }
-        for (int k = 0; k < steps; ++k, ++it) {
+        for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
           if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
             ok = false;
@@ -434,7 +528,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     Tile t;
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t st0 = __shfl_sync(0xffffffffu, smem_addr(stages), 0);
-    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x, ++n) {
+    int k0, k1;
+    bool shared;
+    for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
+      if (k1 == 0) continue;
       if (n >= kBack &&
           !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag))
         ok = false;
@@ -444,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const uint32_t d = base + (n & 1) * C::kAcc1;
-      for (int k = 0; k < steps; ++k, ++it) {
+      for (int k = k0; k < k1; ++k, ++it) {
         const int s = it % S;
         // the scale slot's last reader, two steps back
         if ((it >= 2 && !mbar_wait(&empty[(it - 2) % S], ((it - 2) / S) & 1, abort_flag)) ||
@@ -463,15 +560,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t sd = scale_desc(st + kABytes + C::kBBytes);
         const int mmas = min(4, (p.K - k * kStepCols + 63) / 64);
         if (elect_one()) {
-          if (mmas == 4) issue_step<kFormat, BN, 4>(d, ad, bd, sd, sfa, sfb, k != 0);
-          else if (mmas == 3) issue_step<kFormat, BN, 3>(d, ad, bd, sd, sfa, sfb, k != 0);
-          else if (mmas == 2) issue_step<kFormat, BN, 2>(d, ad, bd, sd, sfa, sfb, k != 0);
-          else issue_step<kFormat, BN, 1>(d, ad, bd, sd, sfa, sfb, k != 0);
+          if (mmas == 4) issue_step<kFormat, BN, kSplit, 4>(d, ad, bd, sd, sfa, sfb, k != k0);
+          else if (mmas == 3) issue_step<kFormat, BN, kSplit, 3>(d, ad, bd, sd, sfa, sfb, k != k0);
+          else if (mmas == 2) issue_step<kFormat, BN, kSplit, 2>(d, ad, bd, sd, sfa, sfb, k != k0);
+          else issue_step<kFormat, BN, kSplit, 1>(d, ad, bd, sd, sfa, sfb, k != k0);
           tc_commit(&empty[s]);
-          if (k == steps - 1) tc_commit(&tfull[n & 1]);
+          if (k == k1 - 1) tc_commit(&tfull[n & 1]);
         }
         __syncwarp();
       }
+      ++n;
     }
     if (!ok && lane == 0) {
       atomicOr(err, kErrTimeoutMma);
@@ -496,7 +594,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int n = 0;
     bool ok = true;
     Tile t;
-    for (int64_t i = blockIdx.x; ok && tile_of(p, s_first, s_count, i, t); i += gridDim.x, ++n) {
+    uint32_t shared_tiles = 0;  // tiles that the cluster shared so far
+    int k0, k1;
+    bool shared;
+    for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
+      if (k1 == 0) continue;
       if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
         ok = false;
         break;
@@ -509,16 +611,123 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = p.gb ? ga * p.gb[t.e] : ga;
       if (p.row_w && row < t.rows) alpha *= p.row_w[m];
       const int n0 = t.n * BN;
-      if constexpr (kEpi == kSwiglu) {
+      if (kSplit > 1 && shared) {
+        // ---- a tile that the cluster shares: rows 0..31, so only the warps of lanes 0..31
+        constexpr int V = C::kSlice, F = V / 2;  // F: features of a slice (swiglu)
+        auto column = [](int s, int c) {         // the first column of a slice's chunk c of 32
+          if (kEpi != kSwiglu) return s * V + 32 * c;
+          return c < F / 32 ? s * F + 32 * c : 128 + s * F + 32 * (c - F / 32);
+        };
+        const bool mine = q == 0 && (int)rank / (kSplit / 2) == half;
+        // (only warps that send wait for the slot: the others could fall two phases behind)
+        if (q == 0 && (kSplit > 2 || !mine)) {
+          if (shared_tiles > 0 && !mbar_wait_cluster(xfree, (shared_tiles - 1) & 1, abort_flag))
+            ok = false;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int j = 0; j < kSplit / 2; ++j) {
+            const int s = half * (kSplit / 2) + j;
+            if (s == (int)rank) continue;
+            const uint32_t src = rank < (uint32_t)s ? rank : rank - 1;
+            const uint32_t to =
+                peer_addr(smem_addr(exchange), s) + src * (V * 128) + (uint32_t)lane * 16;
+#pragma unroll
+            for (int c = 0; c < V / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld_32x32b<32>(acc + column(s, c), v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                peer_store(to + (c * 8 + x) * 512, v[4 * x], v[4 * x + 1], v[4 * x + 2],
+                           v[4 * x + 3]);
+            }
+            peer_arrive(peer_addr(smem_addr(xfull), s));
+          }
+        }
+        if (mine) {
+          if (!mbar_wait_cluster(xfull, shared_tiles & 1, abort_flag)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          // chunk c of this CTA's slice: the ranks' parts added in their order
+          auto total = [&](int c, uint32_t (&v)[32]) {
+            tmem_ld_32x32b<32>(acc + column((int)rank, c), v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              float sum[4] = {};
+#pragma unroll
+              for (int r = 0; r < kSplit; ++r) {
+                float4 f;
+                if (r == (int)rank) {
+                  f = make_float4(__uint_as_float(v[4 * x]), __uint_as_float(v[4 * x + 1]),
+                                  __uint_as_float(v[4 * x + 2]), __uint_as_float(v[4 * x + 3]));
+                } else {
+                  const int src = r < (int)rank ? r : r - 1;
+                  f = *reinterpret_cast<const float4*>(exchange + src * (V * 128) +
+                                                       (c * 8 + x) * 512 + lane * 16);
+                }
+                sum[0] += f.x;
+                sum[1] += f.y;
+                sum[2] += f.z;
+                sum[3] += f.w;
+              }
+#pragma unroll
+              for (int y = 0; y < 4; ++y) v[4 * x + y] = __float_as_uint(sum[y]);
+            }
+          };
+          if constexpr (kEpi == kSwiglu) {
+            const int I = p.N / 2, c0 = t.n * 128 + (int)rank * F;
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int h = 0; h < F / 32; ++h) {
+              uint32_t gate[32], up[32];
+              total(h, gate);
+              total(F / 32 + h, up);
+              uint4 codes;
+              const uint32_t b = swiglu32<kFormat>(gate, up, alpha, divisor, codes);
+              bytes |= b << (kFormat == FMOE_MXFP4 ? 8 * h : 16 * h);
+              if (row < t.rows)
+                *reinterpret_cast<uint4*>(p.codes + m * (I / 2) + c0 / 2 + 16 * h) = codes;
+            }
+            if (row < t.rows) {
+              const int block = c0 / block_of(kFormat);
+              uint8_t* sc = p.scales +
+                            ((int64_t)t.m * tiles_across(I, kFormat) + block / 4) * kTileBytes +
+                            scale_offset(row, block);
+              if (kFormat == FMOE_MXFP4) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)bytes;
+              else *reinterpret_cast<uint32_t*>(sc) = bytes;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < V / 32; ++c) {
+              uint32_t v[32];
+              total(c, v);
+              store32(p, m0, rows, n0 + column((int)rank, c), v, alpha, wide);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < kSplit; ++r)
+            if (r != (int)rank) peer_arrive(peer_addr(smem_addr(xfree), r));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[n & 1]);
+        ++shared_tiles;
+      } else if constexpr (kEpi == kSwiglu) {
         // this warp's 64 gate columns (col) and 64 up columns (128 + col). The side that lies in
         // the columns shared with the next tile comes first: up in the first accumulator
         // (160..255), gate in the second (0..95).
         const bool first = (n & 1) == 0;
         const uint32_t col = half * 64;
         uint32_t s0[32], s1[32], o[32];
-        const uint32_t shared = acc + col + (first ? 128 : 0), other = acc + col + (first ? 0 : 128);
-        tmem_ld_32x32b<32>(shared, s0);
-        tmem_ld_32x32b<32>(shared + 32, s1);
+        const uint32_t side = acc + col + (first ? 128 : 0), other = acc + col + (first ? 0 : 128);
+        tmem_ld_32x32b<32>(side, s0);
+        tmem_ld_32x32b<32>(side + 32, s1);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -594,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      ++n;
     }
     if (!ok && lane == 0) {
       atomicOr(err, kErrTimeoutEpilogue);
@@ -609,35 +819,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_dealloc(tmem, 512);
   }
   if (threadIdx.x == 0 && *err != 0 && p.sink) report_device_error(p.sink, *err);
+  if constexpr (kSplit > 1) cluster_sync();  // no peer writes to this CTA's memory any more
 }
 
 struct Maps {
   CUtensorMap a, a32, b;
 };
 
-template <int kFormat, int BN, Epilogue kEpi>
-cudaError_t launch(const Maps& maps, const GemmFp4Args& p, int grid, cudaStream_t stream) {
-  auto* fn = fp4_gemm_kernel<kFormat, BN, kEpi>;
+template <int kFormat, int BN, Epilogue kEpi, int kSplit>
+cudaError_t launch(const Maps& maps, const GemmFp4Args& p, int clusters, cudaStream_t stream) {
+  using C = Cfg<kFormat, BN, kSplit>;
+  auto* fn = fp4_gemm_kernel<kFormat, BN, kEpi, kSplit>;
   static thread_local int configured = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (configured != dev) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg<kFormat, BN>::kSmemBytes);
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) return e;
     configured = dev;
   }
-  return launch_pdl(fn, dim3((unsigned)grid), dim3(kThreads), Cfg<kFormat, BN>::kSmemBytes, stream,
-                    maps.a, maps.a32, maps.b, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * kSplit));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kSplit;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kSplit > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fn, maps.a, maps.a32, maps.b, p);
 }
 
 template <int kFormat>
-cudaError_t launch(int bn, bool swiglu, const Maps& maps, const GemmFp4Args& p, int grid,
-                   cudaStream_t stream) {
-  if (swiglu) return launch<kFormat, 256, kSwiglu>(maps, p, grid, stream);
-  if (bn == 128) return launch<kFormat, 128, kStore>(maps, p, grid, stream);
-  return launch<kFormat, 256, kStore>(maps, p, grid, stream);
+cudaError_t launch(int bn, int split, bool swiglu, const Maps& maps, const GemmFp4Args& p,
+                   int clusters, cudaStream_t stream) {
+  if (swiglu && split > 1) return launch<kFormat, 256, kSwiglu, 2>(maps, p, clusters, stream);
+  if (swiglu) return launch<kFormat, 256, kSwiglu, 1>(maps, p, clusters, stream);
+  if (bn == 256 && split > 1) return launch<kFormat, 256, kStore, 2>(maps, p, clusters, stream);
+  if (bn == 256) return launch<kFormat, 256, kStore, 1>(maps, p, clusters, stream);
+  if (split == 4) return launch<kFormat, 128, kStore, 4>(maps, p, clusters, stream);
+  if (split == 2) return launch<kFormat, 128, kStore, 2>(maps, p, clusters, stream);
+  return launch<kFormat, 128, kStore, 1>(maps, p, clusters, stream);
 }
 
 int bad(const std::string& msg) {
@@ -667,10 +895,21 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
   p.scales = static_cast<uint8_t*>(g.scales);
   p.gc = g.gc;
   p.m_tiles = (int)tiles_down(g.M);
-  // the widest tile that still gives every SM one
   const bool swiglu = g.codes != nullptr;
-  int bn = 256;
-  while (!swiglu && bn > 128 && (int64_t)p.m_tiles * ((g.N + bn - 1) / bn) < sms) bn /= 2;
+  const int steps = (g.K + kStepCols - 1) / kStepCols;
+  int bn = 256, split = 1;
+  if (g.experts == 0) {
+    // the widest tile that still gives every SM one; few rows and too few tiles for that: tiles
+    // shared by 2 or 4 CTAs, as long as each has two K steps or more
+    while (bn > 128 && (int64_t)p.m_tiles * ((g.N + bn - 1) / bn) < sms) bn /= 2;
+    if (g.M <= 32 && bn == 128) {
+      const int tiles = (g.N + bn - 1) / bn;
+      while (split < 4 && tiles * split * 2 <= sms && steps >= 4 * split) split *= 2;
+    }
+  } else if (g.few_rows && steps >= 4) {
+    // an expert's few rows make one row tile: half tiles even out the last wave
+    split = 2;
+  }
   p.n_tiles = (g.N + bn - 1) / bn;
   p.panel = 8;
   p.sink = device_error_sink(stream);
@@ -681,10 +920,10 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
     v = make_byte_map(&maps.b, g.b, g.K / 2, g.N, g.experts > 0 ? g.experts : 1, 128, 128, "b");
   if (v != FMOE_OK) return v;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  const int grid = (int)(tiles < sms ? tiles : sms);
+  const int clusters = (int)(tiles < sms / split ? tiles : sms / split);
   const cudaError_t e = g.format == FMOE_MXFP4
-                            ? launch<FMOE_MXFP4>(bn, swiglu, maps, p, grid, stream)
-                            : launch<FMOE_NVFP4>(bn, swiglu, maps, p, grid, stream);
+                            ? launch<FMOE_MXFP4>(bn, split, swiglu, maps, p, clusters, stream)
+                            : launch<FMOE_NVFP4>(bn, split, swiglu, maps, p, clusters, stream);
   if (e == cudaSuccess) return FMOE_OK;
   set_last_error(std::string("4-bit product: ") + cudaGetErrorString(e));
   return FMOE_ERR_RUNTIME;

@@ -140,7 +140,8 @@ def _close(got, a, b, dtype):
 @pytest.mark.parametrize("M,N,K", [
     (1, 1, 32), (1, 128, 256), (7, 40, 64), (16, 4096, 512), (33, 129, 96), (128, 256, 1024),
     (129, 255, 2080), (300, 300, 288), (1, 5000, 7168), (257, 1, 160), (64, 520, 4128),
-    (1500, 3400, 1056), (4999, 1057, 288), (200, 19000, 544)])
+    (1500, 3400, 1056), (4999, 1057, 288), (200, 19000, 544),
+    (16, 300, 2080), (7, 4096, 1024), (32, 1000, 4128), (1, 8, 1056), (31, 9000, 2048)])
 def test_matmul(fmoe, fmt, M, N, K):
     ca, sa, a = _operand(M, K, fmt, None, M + K)
     cb, sb, b = _operand(N, K, fmt, None, N + K + 1)

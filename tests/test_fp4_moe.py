@@ -105,6 +105,8 @@ def _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, seed, offset=0, route="rando
         idx[torch.rand(T, K, generator=g) < 0.4] = -1
     elif route == "one":
         idx[:] = offset + 1
+    elif route == "skewed":
+        idx[: T * 2 // 3, 0] = offset + 2
     elif route == "none":
         idx[:] = -1
     w = torch.rand(T, K, generator=g) - 0.2
@@ -132,6 +134,11 @@ def _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, seed, offset=0, route="rando
     (9, 256, 128, 8, 8, 2, 0, "none", torch.bfloat16),
     (2000, 128, 128, 256, 256, 8, 0, "random", torch.bfloat16),
     (50, 1056, 384, 5, 3, 5, 1, "random", torch.float32),
+    # few rows an expert and long sums: tiles shared by two CTAs, next to an expert of more rows
+    (16, 1056, 1152, 16, 16, 4, 0, "random", torch.bfloat16),
+    (1, 2048, 1024, 8, 8, 2, 0, "random", torch.bfloat16),
+    (60, 1280, 1152, 16, 8, 2, 3, "skewed", torch.bfloat16),
+    (33, 1024, 1056, 64, 64, 8, 0, "holes", torch.float16),
 ])
 def test_forward_fp4(fmoe, fmt, T, H, I, E, E_local, K, offset, route, dtype):
     args, kw, state = _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, T + H, offset, route)
