@@ -7,8 +7,9 @@
 //
 // A CTA (one per SM, persistent) computes tiles of 128 rows of a by BN rows of b. K steps of 256
 // values: 128 bytes of codes a row (one 128-byte swizzle row) and the scale tiles of those 256
-// columns, which lie back to back in memory (fp4.cuh). Warp 0 issues the copies, warp 1 the
-// scale copies into tensor memory and the MMAs (4 of K = 64 a step), warps 2..9 store tiles.
+// columns, which lie back to back in memory (fp4.cuh). Warp 0 issues b's copies and warp 10 those
+// of a (a copy costs its thread about 90 cycles, a step has 6), warp 1 the scale copies into tensor
+// memory and the MMAs (4 of K = 64 a step), warps 2..9 store tiles.
 // Scale columns in tensor memory have two slots: the copies for step k + 2 are issued when the
 // MMAs of step k have retired. A scale operand starts at a whole scale tile (4 columns), so BN
 // is a multiple of 128.
@@ -40,7 +41,7 @@ namespace {
 using namespace fp4;
 using namespace sm100;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr int kEpiWarps = 8;
 constexpr int kStepCols = 256;      // K values per step
 constexpr int kABytes = 128 * 128;
@@ -182,6 +183,7 @@ struct GemmFp4Args {
   uint8_t* codes;
   uint8_t* scales;
   const float* gc;
+  bool early;
   unsigned* sink;
 };
 
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);  // the issuers of a and of b
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -421,14 +423,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-  pdl_trigger();
+  // Within the expert layer (p.early) the plan and the weights were complete before the kernel in
+  // front of this one passed its own wait, which this grid starts behind: the weights' copies
+  // need not wait for it.
+  if (!p.early) {
+    pdl_wait();
+    pdl_trigger();
+  }
   if (p.experts > 0) {
     for (int e = threadIdx.x; e <= p.experts; e += kThreads) {
       s_first[e] = p.tile_first[e];
       if (e < p.experts) s_count[e] = p.count[e];
     }
     __syncthreads();
+  }
+  if (p.early && warp != 0) {
+    pdl_wait();
+    pdl_trigger();
   }
 
   const int steps = (p.K + kStepCols - 1) / kStepCols;
@@ -464,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      // ------------------------------------------------------------------ copies
-      const uint64_t keep = policy_evict_last();
+      // ------------------------------------------------------------------ copies of b
+      const uint64_t keep = policy_evict_last(), once = policy_evict_first();
       int it = 0;
       bool ok = true;
       Tile t;
@@ -473,7 +484,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool shared;
       for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
         if (k1 == 0) continue;
-        const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
         // the 128-row runs of b: next to each other, or gate and up rows
         int row[C::kRuns], runs = 0;
         const uint8_t* sb[C::kRuns];
@@ -483,6 +493,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (row[r] < p.N) ++runs;  // a run past b's last row is not there
           sb[r] = p.sb + ((int64_t)t.e * tiles_down(p.N) + row[r] / 128) * across * kTileBytes;
         }
+        // an expert with one row tile reads its weights once
+        const bool reread = p.experts == 0 || s_first[t.e + 1] - s_first[t.e] > 1;
+        const uint64_t policy = reread ? keep : once;
         for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % S;
           if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
@@ -493,28 +506,61 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* sc = st + kABytes + C::kBBytes;
           const int have = min(C::kScaleTiles, across - k * C::kScaleTiles) * kTileBytes;
           const int64_t at = (int64_t)k * C::kScaleTiles * kTileBytes;
-          // few rows: boxes of 32 (the other rows of the stage keep what they held; a row of a
-          // only reaches its own row of the product)
-          const int boxes = t.rows > 64 ? 0 : (t.rows + 31) / 32;
-          mbar_arrive_expect_tx(&full[s], (boxes ? boxes * 4096 : kABytes) + have +
-                                              runs * (128 * 128 + have));
+          mbar_arrive_expect_tx(&full[s], runs * (128 * 128 + have));
 #pragma unroll
           for (int r = 0; r < C::kRuns; ++r) {
             if (r >= runs) break;
-            tma_load_3d(st + kABytes + r * 128 * 128, &map_b, &full[s], k * 128, row[r], t.e, keep);
+            tma_load_3d(st + kABytes + r * 128 * 128, &map_b, &full[s], k * 128, row[r], t.e,
+                        policy);
             bulk_load_1d(sc + (1 + r) * C::kRunBytes, sb[r] + at, have, &full[s]);
           }
-          if (boxes == 0) tma_load_2d(st, &map_a, &full[s], k * 128, t.m * 128, keep);
-          for (int x = 0; x < boxes; ++x)
-            tma_load_2d(st + x * 4096, &map_a32, &full[s], k * 128, t.m * 128 + 32 * x, keep);
-          bulk_load_1d(sc, sa + at, have, &full[s]);
         }
       }
       if (!ok) {
         atomicOr(err, kErrTimeoutProducer);
         *abort_flag = 1;
       }
-      // every issued copy must land before the CTA's shared memory is released
+      // every copy must land before the CTA's shared memory is released (where the other issuer
+      // gave up, the wait runs out: the copies have landed by then)
+      static const int zero = 0;
+      for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&full[j % S], (j / S) & 1, &zero);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ copies of a
+      const uint64_t keep = policy_evict_last();
+      int it = 0;
+      bool ok = true;
+      Tile t;
+      int k0, k1;
+      bool shared;
+      for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
+        if (k1 == 0) continue;
+        const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
+        // few rows: boxes of 32 (the other rows of the stage keep what they held; a row of a
+        // only reaches its own row of the product)
+        const int boxes = t.rows > 64 ? 0 : (t.rows + 31) / 32;
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = stages + s * C::kStageBytes;
+          const int have = min(C::kScaleTiles, across - k * C::kScaleTiles) * kTileBytes;
+          mbar_arrive_expect_tx(&full[s], (boxes ? boxes * 4096 : kABytes) + have);
+          if (boxes == 0) tma_load_2d(st, &map_a, &full[s], k * 128, t.m * 128, keep);
+          for (int x = 0; x < boxes; ++x)
+            tma_load_2d(st + x * 4096, &map_a32, &full[s], k * 128, t.m * 128 + 32 * x, keep);
+          bulk_load_1d(st + kABytes + C::kBBytes, sa + (int64_t)k * C::kScaleTiles * kTileBytes,
+                       have, &full[s]);
+        }
+      }
+      if (!ok) {
+        atomicOr(err, kErrTimeoutProducer);
+        *abort_flag = 1;
+      }
       static const int zero = 0;
       for (int j = it > S ? it - S : 0; j < it; ++j) mbar_wait(&full[j % S], (j / S) & 1, &zero);
     }
@@ -894,6 +940,7 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
   p.codes = static_cast<uint8_t*>(g.codes);
   p.scales = static_cast<uint8_t*>(g.scales);
   p.gc = g.gc;
+  p.early = g.early;
   p.m_tiles = (int)tiles_down(g.M);
   const bool swiglu = g.codes != nullptr;
   const int steps = (g.K + kStepCols - 1) / kStepCols;
@@ -906,9 +953,6 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
       const int tiles = (g.N + bn - 1) / bn;
       while (split < 4 && tiles * split * 2 <= sms && steps >= 4 * split) split *= 2;
     }
-  } else if (g.few_rows && steps >= 4) {
-    // an expert's few rows make one row tile: half tiles even out the last wave
-    split = 2;
   }
   p.n_tiles = (g.N + bn - 1) / bn;
   p.panel = 8;

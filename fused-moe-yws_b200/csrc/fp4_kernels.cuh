@@ -50,7 +50,8 @@ struct Fp4Gemm {
   const int* tile_first;  // [experts + 1] on the device
   const int* count;       // [experts] on the device
   const float* row_w;     // or null: factor of each row of out
-  bool few_rows;          // grouped: most experts have at most 32 rows
+  bool early;             // b, tile_first and count were complete before the kernel in front of
+                          // this one on the stream passed its dependency wait
   // Or, instead of out: b's rows are N / 2 gate and N / 2 up rows (N / 2 a multiple of 128), and
   // gate * silu(up) goes to a 4-bit matrix [M, N / 2] with the global scale gc (null: 1).
   void* codes;

@@ -303,7 +303,7 @@ extern "C" int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensor
   g.ga = t->input_scale;
   g.gb = t->w13_global;
   g.experts = E;
-  g.few_rows = plan.pairs <= 32 * (int64_t)E;
+  g.early = true;
   g.tile_first = plan.tile_first;
   g.count = plan.count;
   if (fused(p)) {
