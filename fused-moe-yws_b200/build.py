@@ -7,6 +7,7 @@ Produces, inside ``fused-moe-yws_b200/lib``:
   relies on IEEE single-precision rounding).
 * ``libfmoe_tvm_ffi.so`` -- the TVM-FFI ``kernel`` export with the reference signature,
   built only when the ``tvm_ffi`` headers are importable.
+* ``fmoe_torch.so`` -- the compiled Python entry points of the router and the 4-bit operators.
 
 Run ``python fused-moe-yws_b200/build.py`` or call ``build()``.
 """
@@ -93,9 +94,33 @@ def build_tvm_ffi(verbose: bool = False):
     return so
 
 
+def build_torch(verbose: bool = False) -> Path:
+    """The compiled Python entry points of the router and the 4-bit operators (fmoe_torch.so)."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    src = CSRC / "torch_binding.cpp"
+    so = LIB / "fmoe_torch.so"
+    if _stale(so, [src, INCLUDE / "fmoe.h", LIB / "libfmoe.so"]):
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", str(src), "-o",
+               str(so), f"-I{INCLUDE}", f"-I{CUDA_HOME / 'include'}", f"-I{root / 'include'}",
+               f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+               f"-I{sysconfig.get_paths()['include']}",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f"-L{LIB}", "-lfmoe", f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+               "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{root / 'lib'}"]
+        subprocess.check_call(cmd)
+        if verbose:
+            print(f"[fmoe build] linked {so}")
+    return so
+
+
 def build(verbose: bool = False):
     so = build_core(verbose)
     tvm = build_tvm_ffi(verbose)
+    build_torch(verbose)
     return so, tvm
 
 

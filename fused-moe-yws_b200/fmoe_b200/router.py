@@ -8,21 +8,21 @@ differentiable.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 
 import torch
 
-from . import FMOE_OK, FmoeRouteOut, _check_tensor, _raise, load_library
+from . import LIB_PATH, load_library
 
-# the current stream's handle without a Stream object around it (half the host time of a call)
-_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"top2": 0, "max": 1}
+_module = None
 
 
 class FmoeRouter(ctypes.Structure):
+    """The C argument block, for callers of the C ABI (fmoe_route_experts) through ctypes."""
+
     _fields_ = [("num_tokens", ctypes.c_int64), ("logits_stride", ctypes.c_int64),
                 ("num_experts", ctypes.c_int32), ("top_k", ctypes.c_int32),
                 ("n_group", ctypes.c_int32), ("topk_group", ctypes.c_int32),
@@ -31,76 +31,33 @@ class FmoeRouter(ctypes.Structure):
                 ("bias_dtype", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
-def _code(table, value, name):
+def binding():
+    """The compiled entry points (lib/fmoe_torch.so, csrc/torch_binding.cpp)."""
+    global _module
+    if _module is None:
+        load_library()
+        path = LIB_PATH.with_name("fmoe_torch.so")
+        if not path.exists():
+            raise RuntimeError(f"torch binding not built: {path} (run `python "
+                               f"fused-moe-yws_b200/build.py`)")
+        loader = importlib.machinery.ExtensionFileLoader("fmoe_torch", str(path))
+        spec = importlib.util.spec_from_file_location("fmoe_torch", path, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _module = module
+    return _module
+
+
+def code(table, value, name):
     if value not in table:
         raise ValueError(f"{name} must be one of {', '.join(table)}, got {value!r}")
     return table[value]
 
 
-def _expect(t, name, shape, dtype, dev):
-    """_check_tensor and the device, in one test for the arguments that are as they should be."""
-    if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype
-            and t.device == dev and t.is_contiguous()):
-        _check_tensor(t, name, shape, dtype)
-        raise ValueError(f"{name} must be on {dev}, got {t.device}")
-
-
-def _call(where, dev, name, *args):
-    """The library's function `name` on dev's current stream; raises what it reports."""
-    lib = load_library()
-    if dev.index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, _stream_handle(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            rc = getattr(lib, name)(*args, _stream_handle(dev.index))
-    if rc != FMOE_OK:
-        _raise(lib, rc, where)
-
-
-def _logits(logits):
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
-        raise ValueError("logits must be 2D")
-    if logits.device.type != "cuda":
-        raise ValueError("logits must be a CUDA tensor")
-    if logits.dtype not in DTYPE_CODES:
-        raise TypeError(f"logits dtype mismatch: expected float32, bfloat16 or float16, got "
-                        f"{logits.dtype}")
-    # rows may be padded; anything else (transposed, broadcast) is laid out first
-    E = logits.shape[1]
-    if logits.stride(1) != 1 and E > 1 or logits.stride(0) < E and logits.shape[0] > 1:
-        logits = logits.contiguous()
-    return logits
-
-
-def _router(logits, top_k, score, n_group, topk_group, group_score, renormalize, scale,
-            bias_dtype=torch.float32):
-    T, E = logits.shape
-    return FmoeRouter(T, logits.stride(0) if T > 1 else E, E, int(top_k), int(n_group),
-                      int(topk_group), _code(_SCORES, score, "score"),
-                      _code(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)),
-                      DTYPE_CODES[logits.dtype], DTYPE_CODES[bias_dtype], float(scale))
-
-
 def _forward(logits, bias, top_k, score, n_group, topk_group, group_score, renormalize, scale):
-    logits = _logits(logits)
-    T, E = logits.shape
-    bias_dtype = torch.float32
-    if bias is not None:
-        if not isinstance(bias, torch.Tensor):
-            raise ValueError("bias must be a torch.Tensor")
-        bias_dtype = bias.dtype
-        if bias_dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError(f"bias dtype mismatch: expected float32 or bfloat16, got {bias_dtype}")
-        _expect(bias, "bias", (E,), bias_dtype, logits.device)
-    r = _router(logits, top_k, score, n_group, topk_group, group_score, renormalize, scale,
-                bias_dtype)
-    dev = logits.device
-    idx = torch.empty(T, max(int(top_k), 0), dtype=torch.int32, device=dev)
-    w = torch.empty(T, max(int(top_k), 0), dtype=torch.float32, device=dev)
-    out = FmoeRouteOut(idx.data_ptr(), w.data_ptr())
-    _call("route_experts", dev, "fmoe_route_experts", ctypes.byref(r), logits.data_ptr(),
-          None if bias is None else bias.data_ptr(), ctypes.byref(out))
-    return idx, w
+    return (_module or binding()).route_experts(
+        logits, top_k, code(_SCORES, score, "score"), bias, n_group, topk_group,
+        code(_GROUP_SCORES, group_score, "group_score"), renormalize, scale)
 
 
 def route_experts_backward(grad_w: torch.Tensor, logits: torch.Tensor, topk_idx: torch.Tensor, *,
@@ -110,21 +67,8 @@ def route_experts_backward(grad_w: torch.Tensor, logits: torch.Tensor, topk_idx:
     ``topk_idx`` [T, K] are the picks of ``route_experts``, ``grad_w`` fp32 [T, K]; ``score``,
     ``renormalize`` and ``scale`` as there (groups and bias only decide the picks). Returns
     [T, E] in the logits' type."""
-    logits = _logits(logits)
-    T, E = logits.shape
-    if not isinstance(topk_idx, torch.Tensor) or topk_idx.dim() != 2:
-        raise ValueError("topk_idx must be 2D")
-    K = topk_idx.shape[1]
-    dev = logits.device
-    _expect(topk_idx, "topk_idx", (T, K), torch.int32, dev)
-    if isinstance(grad_w, torch.Tensor):
-        grad_w = grad_w.contiguous()  # a gradient may arrive broadcast
-    _expect(grad_w, "grad_w", (T, K), torch.float32, dev)
-    r = _router(logits, K, score, 1, 1, "top2", renormalize, scale)
-    out = torch.empty(T, E, dtype=logits.dtype, device=dev)
-    _call("route_experts_backward", dev, "fmoe_route_experts_backward", ctypes.byref(r),
-          grad_w.data_ptr(), logits.data_ptr(), topk_idx.data_ptr(), out.data_ptr())
-    return out
+    return (_module or binding()).route_experts_backward(
+        grad_w, logits, topk_idx, code(_SCORES, score, "score"), renormalize, scale)
 
 
 class _RouteExperts(torch.autograd.Function):
