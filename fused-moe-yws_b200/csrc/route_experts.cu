@@ -233,18 +233,26 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
   return r;
 }
 
+// An expert's biased sigmoid score in 64 bits. Not inlined: tokens that need it are rare, and
+// their warp waits for the code.
+__device__ __noinline__ double exact_score(float x, float bias) {
+  return 1.0 / (1.0 + exp(-(double)x)) + (double)bias;
+}
+
 // Picks by one 32-bit key an expert: its value in the high bits, its index (reversed, so that
 // the lower index wins a tie) in the low ones. A lane sorts its keys once; a round is one warp
 // maximum and a shift in the winning lane.
-//   bias     the score on a grid over the row's range, 23 bits for up to 512 experts; false
-//            where two scores that matter are not told apart (see select_experts: tol is twice
-//            a score's error, the grid adds two steps for its roundings)
+//   bias     the score on a grid over the row's range, 23 bits for up to 512 experts (see
+//            select_experts: tol is twice a score's error, the grid adds two steps for its
+//            roundings). Where two sigmoid scores that matter are not told apart, those alone are
+//            taken in 64 bits; where that does not do (a softmax needs its whole row; the
+//            runner-up is near too) the result is false.
 //   no bias  16-bit logits as they are: exact
 // Groups are whole runs of lanes, or there are none. Issue-bound: 1150 instructions a token
 // with compared (value, index) pairs, 28 us for 16384 x 256 on B200.
 template <int EPL, typename In>
-__device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (&x)[EPL], int lane,
-                                              int& pick) {
+__device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
+                                              const float (&x)[EPL], int lane, int& pick) {
   constexpr int kScoreBits = EPL <= 8 ? 8 : EPL == 16 ? 9 : 10;  // index bits beside a score
   const int e0 = lane * EPL;
   uint32_t p[EPL];
@@ -332,7 +340,11 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (
     }
   }
   sort_keys(p);
-  bool sure = true;
+  const uint32_t mask = (1u << bits) - 1;
+  auto exact = [&](int e) {
+    return exact_score(to_float(static_cast<const In*>(a.logits)[t * a.stride + e]),
+                       load_bias(a, e));
+  };
   if (a.n_group > 1) {
     const int span = 32 / a.n_group, own = lane / span;
     uint32_t m1 = p[0] >> bits, m2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] >> bits : 0u;
@@ -351,11 +363,38 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (
       rank += h < a.n_group && (v > mine || (v == mine && h < own));
     }
     for (int o = 1; o < span; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
-    const bool keep = rank < a.topk_group;
+    bool keep = rank < a.topk_group;
     if (near) {
       const uint32_t worst = __reduce_min_sync(kAll, keep ? mine : 0xffffffffu);
       const uint32_t best = __reduce_max_sync(kAll, keep ? 0u : mine);
-      if (best > 0 && worst - best <= 2 * near) sure = false;
+      if (best > 0 && worst - best <= 2 * near) {
+        // the groups' scores again, from their two best experts in 64 bits
+        if (a.softmax) return false;
+        uint32_t b1 = p[0], b2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] : 0u;
+        uint32_t b3 = EPL > 2 ? p[EPL > 2 ? 2 : 0] : 0u;
+        for (int o = 1; o < span; o <<= 1) {
+          const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
+          const uint32_t q3 = __shfl_xor_sync(kAll, b3, o);
+          // the three largest of two descending triples
+          const uint32_t low = min(b1, q1), mid = max(b2, q2);
+          b3 = max(max(min(low, mid), b3), max(q3, min(b2, q2)));
+          b2 = max(low, mid);
+          b1 = max(b1, q1);
+        }
+        const uint32_t last = a.group_max ? b1 : b2, after = a.group_max ? b2 : b3;
+        if (__any_sync(kAll, last && after && (last >> bits) - (after >> bits) <= near)) return false;
+        double score = (double)neg_inf();
+        if (last) {
+          score = exact((int)(mask - (b1 & mask)));
+          if (!a.group_max) score += exact((int)(mask - (b2 & mask)));
+        }
+        rank = 0;
+        for (int h = 0; h < a.n_group; ++h) {
+          const double v = __shfl_sync(kAll, score, h * span);
+          rank += v > score || (v == score && h < own);
+        }
+        keep = rank < a.topk_group;
+      }
     }
     if (!keep) {
 #pragma unroll
@@ -363,24 +402,43 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, const float (
     }
   }
   pick = -1;
-  const uint32_t mask = (1u << bits) - 1;
   uint32_t gap = 0xffffffffu, last = 0;  // smallest distance of neighbours in the order
   const int rounds = a.K + (near ? 1 : 0);
-  for (int k = 0; k < rounds; ++k) {
+  int found = 0;
+  for (; found < rounds; ++found) {
     const uint32_t top = __reduce_max_sync(kAll, p[0]);
     if (top == 0) break;  // fewer usable experts than top_k
-    if (k > 0) gap = min(gap, last - top);
+    if (found > 0) gap = min(gap, last - top);
     last = top;
-    if (lane == k) pick = (int)(mask - (top & mask));
+    if (lane == found) pick = (int)(mask - (top & mask));
     if (p[0] == top) {
 #pragma unroll
       for (int j = 0; j + 1 < EPL; ++j) p[j] = p[j + 1];
       p[EPL - 1] = 0u;
     }
   }
+  if (near && (gap >> bits) <= near) {
+    // the picks and the runner-up in 64 bits, put in order by counting; the one behind them has to
+    // be clear of them
+    const uint32_t behind = __reduce_max_sync(kAll, p[0]);
+    if (a.softmax || found > 32 || (behind && (last >> bits) - (behind >> bits) <= near))
+      return false;
+    const double score = pick >= 0 ? exact(pick) : 0.0;
+    int rank = 0;
+    for (int k = 0; k < found; ++k) {
+      const double v = __shfl_sync(kAll, score, k);
+      const int e = __shfl_sync(kAll, pick, k);
+      rank += v > score || (v == score && e < pick);
+    }
+    int ordered = -1;
+    for (int k = 0; k < found; ++k) {
+      const int to = __shfl_sync(kAll, rank, k), e = __shfl_sync(kAll, pick, k);
+      if (lane == to) ordered = e;
+    }
+    pick = ordered;
+  }
   if (lane >= a.K) pick = -1;
-  if (near && (gap >> bits) <= near) sure = false;
-  return sure;
+  return true;
 }
 
 // Picks the token's experts: lane k gets the k-th one, or -1. V = float: false where the scores
@@ -570,7 +628,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_kernel(Router
   load_logits<EPL, In>(a, t, lane, x);
   int pick;
   bool sure = false;
-  if (a.by_key && (a.bias || sizeof(In) == 2)) sure = select_by_key<EPL, In>(a, x, lane, pick);
+  if (a.by_key && (a.bias || sizeof(In) == 2)) sure = select_by_key<EPL, In>(a, t, x, lane, pick);
   else sure = select_experts<EPL, float>(a, x, lane, pick);
   if (!sure) select_experts<EPL, double>(a, x, lane, pick);
   float top = 0.0f, sum = 1.0f;

@@ -126,6 +126,31 @@ def test_route_experts_decides_below_single_precision(fmoe, score):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,K,n,kg,how", [(256, 8, 8, 4, "top2"), (256, 8, 8, 3, "max"),
+                                          (64, 6, 2, 1, "top2"), (32, 4, 1, 1, "max"),
+                                          (256, 32, 1, 1, "max"), (1024, 8, 4, 2, "top2")])
+def test_route_experts_crowded_scores(fmoe, score, E, K, n, kg, how):
+    """Logits a few units in the last place apart, so that many scores, group sums and runners-up
+    round alike, in ones, twos and threes; and scores that a bias brings that close."""
+    g = torch.Generator().manual_seed(E + K)
+    T = 60
+    base = torch.randn(T, E, generator=g)
+    x = (base * 2).round() / 2 + torch.randint(-3, 4, (T, E), generator=g) * 2.0 ** -22
+    b = torch.randint(-2, 3, (E,), generator=g) * 2.0 ** -24 + 0.125
+    # expert e + E/2 gets a bias that evens out its score's distance to expert e's
+    far = torch.randn(T, E, generator=g)
+    c = torch.zeros(E)
+    s = torch.sigmoid(far.double())
+    c[E // 2:] = (s[0, :E // 2] - s[0, E // 2:]).float()
+    for logits, bias in ((x, b), (x, None), (far, c)):
+        idx, _ = fmoe.route_experts(logits.cuda(), K, score=score, n_group=n, topk_group=kg,
+                                    group_score=how, bias=None if bias is None else bias.cuda())
+        want, _ = ref.route(logits, bias, K, score, n, kg, how)
+        assert torch.equal(idx.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_experts_infinite_logits(fmoe, score):
     x = torch.randn(4, 32, generator=torch.Generator().manual_seed(0))
     x[0, 7] = math.inf
