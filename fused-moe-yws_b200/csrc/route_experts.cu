@@ -23,6 +23,7 @@
 #include "fmoe.h"
 #include "fmoe_common.cuh"
 #include "fmoe_kernels.cuh"
+#include "sm100.cuh"
 
 namespace fmoe {
 namespace {
@@ -65,14 +66,28 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
-// N consecutive elements, as vectors of up to 16 bytes where `wide` says they are aligned and
+// N consecutive elements, as vectors of up to 32 bytes (a sector) where `wide` says they are aligned and
 // inside the row.
 template <int N, typename T>
 __device__ __forceinline__ void load_n(const T* p, bool wide, int inside, T (&v)[N]) {
   constexpr int kBytes = N * (int)sizeof(T);
   if constexpr (kBytes >= 4) {
     if (wide) {
-      if constexpr (kBytes >= 16) {
+      if constexpr (kBytes >= 32) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+        for (int i = 0; i < kBytes / 4; i += 8) {
+          if (inside > 0) {
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]),
+                           "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                         : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[i + j] = 0;
+          }
+        }
+      } else if constexpr (kBytes >= 16) {
 #pragma unroll
         for (int i = 0; i < kBytes / 16; ++i)
           reinterpret_cast<uint4*>(v)[i] =
@@ -96,7 +111,15 @@ __device__ __forceinline__ void store_n(T* p, bool wide, int inside, const T (&v
   if constexpr (kBytes >= 4) {
     if (wide) {
       if (inside <= 0) return;
-      if constexpr (kBytes >= 16) {
+      if constexpr (kBytes >= 32) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+        for (int i = 0; i < kBytes / 4; i += 8) {
+          const uint32_t x[8] = {w[i],     w[i + 1], w[i + 2], w[i + 3],
+                                 w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
+          sm100::st_global_v8(reinterpret_cast<uint32_t*>(p) + i, x);
+        }
+      } else if constexpr (kBytes >= 16) {
 #pragma unroll
         for (int i = 0; i < kBytes / 16; ++i)
           reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
@@ -620,7 +643,7 @@ __device__ __forceinline__ void row_softmax(const float (&x)[EPL], float& top, f
 }
 
 template <int EPL, typename In>
-__global__ void __launch_bounds__(kRouterWarps * 32) route_experts_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(kRouterWarps * 32, EPL <= 8 ? 4 : 1) route_experts_kernel(RouterArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
   if (t >= a.T) return;
@@ -771,9 +794,9 @@ RouterArgs router_args(const fmoe_router* r, const void* logits) {
 // that lie inside the row or outside of it.
 template <int N, typename In>
 bool vectors(const RouterArgs& a) {
-  const size_t bytes = N * sizeof(In) < 16 ? N * sizeof(In) : 16;
+  const size_t bytes = N * sizeof(In) < 32 ? N * sizeof(In) : 32;
   const size_t bias = a.bias_bf16 ? 2 : 4;
-  const size_t bias_bytes = N * bias < 16 ? N * bias : 16;
+  const size_t bias_bytes = N * bias < 32 ? N * bias : 32;
   return a.E % N == 0 && a.stride % N == 0 && bytes >= 4 && bias_bytes >= 4 &&
          reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
          reinterpret_cast<uintptr_t>(a.grad_logits) % bytes == 0 &&
