@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <type_traits>
 
 #include "fmoe.h"
 #include "fmoe_common.cuh"
@@ -27,6 +28,7 @@ constexpr int kCols = 128;             // columns per CTA
 constexpr int kThreads = 256;
 constexpr int kAcross = kCols / 16;    // threads a row
 constexpr int kDown = kThreads / kAcross;
+static_assert(kDown == 32, "rows 32 apart share their place in a scale tile");
 
 template <typename T>
 __device__ __forceinline__ float as_float(T v);
@@ -98,8 +100,13 @@ __device__ __forceinline__ void store16(T* p, const uint32_t (&w)[4 * sizeof(T)]
   }
 }
 
+template <typename T2>
+__device__ __forceinline__ T2 as_pair(uint32_t w) {
+  return *reinterpret_cast<const T2*>(&w);
+}
+
 // The values, and the bits of the largest magnitude as fp32 (NaN above the infinity above the
-// numbers). 16-bit types are compared two at a time in their own bits, which order the same way.
+// numbers). 16-bit types are compared two at a time.
 template <typename T>
 __device__ __forceinline__ uint32_t unpack16(const Raw<T>& r, float (&v)[16]) {
   if constexpr (sizeof(T) == 4) {
@@ -111,21 +118,23 @@ __device__ __forceinline__ uint32_t unpack16(const Raw<T>& r, float (&v)[16]) {
     }
     return top;
   } else {
-    uint32_t top = 0;
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 top = as_pair<T2>(0u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      top = __vmaxu2(top, r.w[i] & 0x7fff7fffu);
+      top = __hmax2_nan(top, as_pair<T2>(r.w[i] & 0x7fff7fffu));
       const T* e = reinterpret_cast<const T*>(&r.w[i]);
       v[2 * i] = as_float<T>(e[0]);
       v[2 * i + 1] = as_float<T>(e[1]);
     }
-    const uint16_t most = (uint16_t)max(top & 0xffffu, top >> 16);
-    return __float_as_uint(as_float<T>(*reinterpret_cast<const T*>(&most))) & 0x7fffffffu;
+    const T* t = reinterpret_cast<const T*>(&top);
+    return __float_as_uint(as_float<T>(__hmax_nan(t[0], t[1])));
   }
 }
 
 template <int kFormat, typename T, int kAlign, bool kSwiglu = false>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) fp4_quantize_kernel(Fp4QuantArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
+    fp4_quantize_kernel(Fp4QuantArgs a) {
   __shared__ __align__(16) uint8_t s_scale[kCols / tile_cols(kFormat) * kTileBytes];
   const int tid = threadIdx.x;
   const int c0 = blockIdx.y * kCols, e = blockIdx.z;
@@ -142,31 +151,39 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) fp4_quantize
   const int tiles = a.tiles_dev ? *a.tiles_dev : (int)tiles_down(a.rows);
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t m0 = (int64_t)tile * kTileRows;
-    // kRows rows at a time, their loads in flight together. Whole warps stay together: an mxfp4
-    // block belongs to two lanes.
+    // A thread's rows are 32 apart (r = 32 u + tid / 8): kRows of them at a time, their loads in
+    // flight together. Whole warps stay together: an mxfp4 block belongs to two lanes.
     constexpr int kRows = kSwiglu ? 2 : 4;
-    for (int r0 = tid / kAcross; r0 < kTileRows; r0 += kRows * kDown) {
+    const int r = tid / kAcross;
+    const int64_t m = m0 + r;
+    const T* from = x + m * a.row_stride + c;
+    uint8_t* to = codes + m * (a.cols / 2) + c / 2;
+    const int left = c < a.cols ? (int)min((int64_t)kTileRows, a.rows - m) : 0;  // rows from m on
+#pragma unroll
+    for (int g = 0; g < kTileRows / kDown; g += kRows) {
       Raw<T> raw[kRows], second[kSwiglu ? kRows : 1];
       bool mine[kRows];
 #pragma unroll
       for (int u = 0; u < kRows; ++u) {
-        const int64_t m = m0 + r0 + u * kDown;
-        int64_t src = m;
-        if (m < a.rows && a.row_index) src = a.row_index[m];
-        mine[u] = m < a.rows && src >= 0 && c < a.cols;
-        if (kSwiglu) src = m;
+        const int d = (g + u) * kDown;
+        mine[u] = d < left;
+        const T* p = from + d * a.row_stride;
+        if (a.row_index) {
+          const int src = mine[u] ? a.row_index[m + d] : -1;
+          mine[u] = src >= 0;
+          if (!kSwiglu) p = x + src * a.row_stride + c;
+        }
         raw[u] = {};
         if (kSwiglu) second[kSwiglu ? u : 0] = {};
         if (mine[u]) {
-          raw[u] = load16<T, kAlign>(x + src * a.row_stride + c);
-          if constexpr (kSwiglu) second[u] = load16<T, kAlign>(x + src * a.row_stride + a.cols + c);
+          raw[u] = load16<T, kAlign>(p);
+          if constexpr (kSwiglu) second[u] = load16<T, kAlign>(p + a.cols);
         }
       }
 #pragma unroll
       for (int u = 0; u < kRows; ++u) {
-        const int r = r0 + u * kDown;
-        const int block = (c - c0) / block_of(kFormat);
-        uint8_t* scale = s_scale + block / 4 * kTileBytes + scale_offset(r, block);
+        uint8_t* scale = s_scale + tid % kAcross * 16 / block_of(kFormat) / 4 * kTileBytes + r * 16 +
+                         (g + u) * 4 + tid % kAcross * 16 / block_of(kFormat) % 4;
         if (!__any_sync(0xffffffffu, mine[u])) {  // few rows a tile: most warps have none
           *scale = 0;
           continue;
@@ -187,7 +204,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4) fp4_quantize
         uint32_t lo, hi;
         const uint32_t byte = encode16<kFormat>(v, top, divisor, lo, hi);
         if (mine[u])
-          *reinterpret_cast<uint2*>(codes + (m0 + r) * (a.cols / 2) + c / 2) = make_uint2(lo, hi);
+          *reinterpret_cast<uint2*>(to + (int64_t)(g + u) * kDown * (a.cols / 2)) =
+              make_uint2(lo, hi);
         *scale = mine[u] ? (uint8_t)byte : 0;
       }
     }
