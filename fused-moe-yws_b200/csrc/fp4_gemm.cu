@@ -645,17 +645,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool shared;
     for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
       if (k1 == 0) continue;
+      const int row = q * 32 + lane;
+      const int64_t m = (int64_t)t.m * 128 + row, m0 = m - lane;
+      const int rows = t.rows - q * 32;  // of this warp's 32
+      float alpha = p.gb ? ga * p.gb[t.e] : ga;  // (loaded while the tile is multiplied)
+      if (p.row_w && row < t.rows) alpha *= p.row_w[m];
       if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
         ok = false;
         break;
       }
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1) * C::kAcc1 + ((uint32_t)(q * 32) << 16);
-      const int row = q * 32 + lane;
-      const int64_t m = (int64_t)t.m * 128 + row, m0 = m - lane;
-      const int rows = t.rows - q * 32;  // of this warp's 32
-      float alpha = p.gb ? ga * p.gb[t.e] : ga;
-      if (p.row_w && row < t.rows) alpha *= p.row_w[m];
       const int n0 = t.n * BN;
       if (kSplit > 1 && shared) {
         // ---- a tile that the cluster shares: rows 0..31, so only the warps of lanes 0..31
