@@ -103,7 +103,7 @@ def build_torch(verbose: bool = False) -> Path:
     root = Path(torch.__file__).resolve().parent
     src = CSRC / "torch_binding.cpp"
     so = LIB / "fmoe_torch.so"
-    if _stale(so, [src, INCLUDE / "fmoe.h", LIB / "libfmoe.so"]):
+    if _stale(so, [src, INCLUDE / "fmoe.h"]):
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", str(src), "-o",
                str(so), f"-I{INCLUDE}", f"-I{CUDA_HOME / 'include'}", f"-I{root / 'include'}",
                f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",

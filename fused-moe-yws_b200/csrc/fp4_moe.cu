@@ -42,8 +42,8 @@ struct PlanArgs {
 __device__ __forceinline__ int local_expert(const PlanArgs& a, int64_t i) {
   if (i >= a.pairs) return -1;
   const int g = a.idx[i];
-  const int e = g - a.offset;
-  return g >= 0 && e >= 0 && e < a.experts ? e : -1;
+  if (g < a.offset) return -1;
+  return g - a.offset < a.experts ? g - a.offset : -1;
 }
 
 // The CTA's pairs per expert.
@@ -233,6 +233,7 @@ int check(const fmoe_fp4_problem* p) {
   if (p->num_tokens < 0 || p->num_tokens > (int64_t)1 << 20)
     return bad("num_tokens must be in [0, 2^20]");
   if (p->top_k < 1 || p->top_k > 32) return bad("top_k must be in [1, 32]");
+  if (p->local_expert_offset < 0) return bad("local_expert_offset must not be negative");
   if (p->num_local_experts < 1 || p->num_local_experts > kPlanExperts)
     return bad("num_local_experts must be in [1, 256]");
   if (p->hidden_size < 32 || p->hidden_size % 32 != 0 || p->hidden_size > 16384)

@@ -282,7 +282,7 @@ def test_forward_fp4_rejects_arguments(fmoe):
 @pytest.mark.parametrize("field,value", [
     ("num_tokens", -1), ("num_tokens", 2 ** 20 + 1), ("hidden_size", 48), ("hidden_size", 0),
     ("hidden_size", 16416), ("intermediate_size", 100), ("num_local_experts", 0),
-    ("num_local_experts", 257), ("top_k", 0), ("top_k", 33), ("format", 2), ("dtype", 3)])
+    ("num_local_experts", 257), ("local_expert_offset", -1), ("top_k", 0), ("top_k", 33), ("format", 2), ("dtype", 3)])
 def test_fp4_forward_rejects(fmoe, field, value):
     from fmoe_b200.fp4 import FmoeFp4Problem, FmoeFp4Tensors
 
