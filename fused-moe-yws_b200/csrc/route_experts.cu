@@ -43,6 +43,7 @@ struct RouterArgs {
   float scale;
   bool wide;         // rows, bias and gradient rows allow a lane's values to move as vectors
   bool by_key;       // select_by_key takes these groups
+  int span_log2;     // lanes of a group there, 32 / n_group, as a power of two
   int* idx;          // [T, K]
   float* w;          // [T, K]
   // backward
@@ -143,10 +144,13 @@ __device__ __forceinline__ void load_logits(const RouterArgs& a, int64_t t, int 
   const int e0 = lane * EPL;
   alignas(16) In raw[EPL];
   load_n(static_cast<const In*>(a.logits) + t * a.stride + e0, a.wide, a.E - e0, raw);
+  // (NaN is the smaller of the two to fmaxf)
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const float v = e0 + j < a.E ? to_float(raw[j]) : neg_inf();
-    x[j] = v > neg_inf() ? v : neg_inf();
+  for (int j = 0; j < EPL; ++j) x[j] = fmaxf(to_float(raw[j]), neg_inf());
+  if (a.E < EPL * 32) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (e0 + j >= a.E) x[j] = neg_inf();
   }
 }
 
@@ -338,7 +342,7 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
     // (its offset's rounding is the same for every expert) and no conversion.
     constexpr int kGrid = 32 - kScoreBits < 23 ? 32 - kScoreBits : 23;
     const float range = high - low;
-    const float step = (float)((1 << kGrid) - 64) / range;
+    const float step = (float)((1 << kGrid) - 64) * fast_reciprocal(range);
     if (!(range > tol) || !(step < 0x1p60f)) return false;  // infinite, or nothing told apart
     const float offset = __fmaf_rn(-low, step, 0x1p23f + 16.0f);
     if (!(fabsf(offset) < 0x1p25f)) return false;  // a range far from zero: too coarse a sum
@@ -369,7 +373,7 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
                        load_bias(a, e));
   };
   if (a.n_group > 1) {
-    const int span = 32 / a.n_group, own = lane / span;
+    const int span = 1 << a.span_log2, own = lane >> a.span_log2;
     uint32_t m1 = p[0] >> bits, m2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] >> bits : 0u;
     for (int o = 1; o < span; o <<= 1) {
       const uint32_t p1 = __shfl_xor_sync(kAll, m1, o), p2 = __shfl_xor_sync(kAll, m2, o);
@@ -381,8 +385,8 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
     // a group's lanes share the comparisons with the other groups
     int rank = 0;
     for (int i = 0; i < a.n_group; i += span) {
-      const int h = i + lane % span;  // past the last group where there are few
-      const uint32_t v = __shfl_sync(kAll, mine, h * span & 31);
+      const int h = i + (lane & (span - 1));  // past the last group where there are few
+      const uint32_t v = __shfl_sync(kAll, mine, (h << a.span_log2) & 31);
       rank += h < a.n_group && (v > mine || (v == mine && h < own));
     }
     for (int o = 1; o < span; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
@@ -424,22 +428,22 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
       for (int j = 0; j < EPL; ++j) p[j] = 0u;
     }
   }
-  pick = -1;
-  uint32_t gap = 0xffffffffu, last = 0;  // smallest distance of neighbours in the order
+  uint32_t gap = 0xffffffffu, last = 0xffffffffu, won = 0;  // gap: of neighbours in the order
   const int rounds = a.K + (near ? 1 : 0);
   int found = 0;
+#pragma unroll 2
   for (; found < rounds; ++found) {
     const uint32_t top = __reduce_max_sync(kAll, p[0]);
     if (top == 0) break;  // fewer usable experts than top_k
-    if (found > 0) gap = min(gap, last - top);
+    gap = min(gap, last - top);
     last = top;
-    if (lane == found) pick = (int)(mask - (top & mask));
-    if (p[0] == top) {
+    if (lane == found) won = top;
+    const bool mine = p[0] == top;
 #pragma unroll
-      for (int j = 0; j + 1 < EPL; ++j) p[j] = p[j + 1];
-      p[EPL - 1] = 0u;
-    }
+    for (int j = 0; j + 1 < EPL; ++j) p[j] = mine ? p[j + 1] : p[j];
+    p[EPL - 1] = mine ? 0u : p[EPL - 1];
   }
+  pick = won ? (int)(mask - (won & mask)) : -1;
   if (near && (gap >> bits) <= near) {
     // the picks and the runner-up in 64 bits, put in order by counting; the one behind them has to
     // be clear of them
@@ -627,7 +631,7 @@ __device__ __forceinline__ float pick_weight(const RouterArgs& a, int pick, floa
     }
     return pick >= 0 ? exp_below(x, top) / sum : 0.0f;
   }
-  return pick >= 0 ? 1.0f / (1.0f + expf(-x)) : 0.0f;
+  return pick >= 0 ? __frcp_rn(1.0f + expf(-x)) : 0.0f;
 }
 
 template <int EPL>
@@ -660,12 +664,12 @@ __global__ void __launch_bounds__(kRouterWarps * 32, EPL <= 8 ? 4 : 1) route_exp
       pick >= 0 ? to_float(static_cast<const In*>(a.logits)[t * a.stride + pick]) : 0.0f;
   float w = pick_weight(a, pick, xp, top, sum);
   if (a.renorm && !a.softmax) {
-    const float total = warp_sum(w) + 1e-20f;
-    w = w / total;
+    w *= __frcp_rn(warp_sum(w) + 1e-20f);
   }
   if (lane < a.K) {
-    a.idx[t * a.K + lane] = pick;
-    a.w[t * a.K + lane] = w * a.scale;
+    const int64_t at = t * a.K + lane;
+    a.idx[at] = pick;
+    a.w[at] = w * a.scale;
   }
 }
 
@@ -806,6 +810,7 @@ bool vectors(const RouterArgs& a) {
 template <int EPL, typename In>
 void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
   a.wide = vectors<EPL, In>(a);
+  while ((32 >> a.span_log2) > a.n_group) ++a.span_log2;
   a.by_key = a.n_group == 1 || (EPL * 32 == a.E && 32 % a.n_group == 0 && (a.bias || a.group_max));
   const unsigned grid = (unsigned)((a.T + kRouterWarps - 1) / kRouterWarps);
   if (backward)
