@@ -139,6 +139,11 @@ def _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, seed, offset=0, route="rando
     (1, 2048, 1024, 8, 8, 2, 0, "random", torch.bfloat16),
     (60, 1280, 1152, 16, 8, 2, 3, "skewed", torch.bfloat16),
     (33, 1024, 1056, 64, 64, 8, 0, "holes", torch.float16),
+    # fewer tiles than SMs and long sums, of few rows and of many
+    (3, 4096, 2304, 4, 4, 2, 0, "random", torch.bfloat16),
+    (200, 2560, 2176, 2, 2, 1, 0, "random", torch.bfloat16),
+    (140, 2080, 2080, 3, 3, 2, 0, "holes", torch.float32),
+    (500, 2048, 2048, 8, 8, 2, 0, "skewed", torch.bfloat16),
 ])
 def test_forward_fp4(fmoe, fmt, T, H, I, E, E_local, K, offset, route, dtype):
     args, kw, state = _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, T + H, offset, route)
