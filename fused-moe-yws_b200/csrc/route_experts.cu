@@ -9,9 +9,14 @@
 //
 // The order is decided as exact arithmetic decides it: two scores that differ by less than
 // single precision resolves still have an order, and a different pick changes the token's
-// output. Every selection here runs in 64 bits.
+// output. Scores are computed in single precision with a bound on their error; what lies within
+// it of a neighbour that matters is decided in 64 bits.
 //
-// One warp routes one token; lane l holds experts l * EPL .. l * EPL + EPL - 1.
+// One warp routes one token; lane l holds experts l * EPL .. l * EPL + EPL - 1. Small batches are
+// bound by the latency of a warp's chain (3.2 us for one token, launch included), large ones by
+// instruction issue: 16384 x 256 with bias and groups runs 750 instructions a token in 16.5 us,
+// where reading the logits takes 2.6 us. All in 64 bits it took 104 us, with compared (value,
+// index) pairs in place of select_by_key's keys 40 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -275,8 +280,7 @@ __device__ __noinline__ double exact_score(float x, float bias) {
 //            taken in 64 bits; where that does not do (a softmax needs its whole row; the
 //            runner-up is near too) the result is false.
 //   no bias  16-bit logits as they are: exact
-// Groups are whole runs of lanes, or there are none. Issue-bound: 1150 instructions a token
-// with compared (value, index) pairs, 28 us for 16384 x 256 on B200.
+// Groups are whole runs of lanes, or there are none.
 template <int EPL, typename In>
 __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
                                               const float (&x)[EPL], int lane, int& pick) {
