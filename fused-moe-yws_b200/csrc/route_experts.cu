@@ -12,7 +12,10 @@
 // output. Scores are computed in single precision with a bound on their error; what lies within
 // it of a neighbour that matters is decided in 64 bits.
 //
-// One warp routes one token; lane l holds experts l * EPL .. l * EPL + EPL - 1. Small batches are
+// One warp routes one token, a lane holds up to EPL consecutive experts; where the number of
+// groups is a power of two, 32 / n_group lanes hold a group's (Place), so that groups of any size
+// merge by shuffles: 14932 x 160 in 8 groups takes 11 us, 55 where a lane's experts cross groups;
+// with 16384 x 256 the mapping costs 0.5 us of 16. Small batches are
 // bound by the latency of a warp's chain (3.2 us for one token, launch included), large ones by
 // instruction issue: 16384 x 256 with bias and groups runs 750 instructions a token in 16.5 us,
 // where reading the logits takes 2.6 us. All in 64 bits it took 104 us, with compared (value,
@@ -47,8 +50,10 @@ struct RouterArgs {
   bool softmax, group_max, renorm;
   float scale;
   bool wide;         // rows, bias and gradient rows allow a lane's values to move as vectors
+  int span_log2;     // lanes of a run of experts, as a power of two
+  int run;           // experts of a run: a group's where `whole`, else all
+  bool whole;        // runs are groups
   bool by_key;       // select_by_key takes these groups
-  int span_log2;     // lanes of a group there, 32 / n_group, as a power of two
   int* idx;          // [T, K]
   float* w;          // [T, K]
   // backward
@@ -72,90 +77,101 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
-// N consecutive elements, as vectors of up to 32 bytes (a sector) where `wide` says they are aligned and
-// inside the row.
+// The experts of a lane: e0 .. e0 + min(n, EPL) - 1, none where n is not positive.
+struct Place {
+  int e0, n;
+};
+template <int EPL>
+__device__ __forceinline__ Place place_of(const RouterArgs& a, int lane) {
+  const int own = lane >> a.span_log2, at = (lane - (own << a.span_log2)) * EPL;
+  return {own * a.run + at, a.run - at};
+}
+
+// The widest vector that N elements of this size are whole multiples of (32 bytes: a sector).
+__host__ __device__ constexpr int vector_bytes(int bytes) {
+  return bytes % 32 == 0 ? 32 : bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : bytes % 4 == 0 ? 4 : 0;
+}
+
+// A lane's elements of a row; as vectors where `wide` says that they are aligned and that a lane
+// has all N or none (it then reads the row's first ones, which saves a branch).
 template <int N, typename T>
-__device__ __forceinline__ void load_n(const T* p, bool wide, int inside, T (&v)[N]) {
-  constexpr int kBytes = N * (int)sizeof(T);
-  if constexpr (kBytes >= 4) {
+__device__ __forceinline__ void load_n(const T* row, const Place& at, bool wide, T (&v)[N]) {
+  constexpr int kVec = vector_bytes(N * (int)sizeof(T));
+  if constexpr (kVec > 0) {
     if (wide) {
-      if constexpr (kBytes >= 32) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(v);
+      uint32_t* w = reinterpret_cast<uint32_t*>(v);
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(row + (at.n > 0 ? at.e0 : 0));
 #pragma unroll
-        for (int i = 0; i < kBytes / 4; i += 8) {
-          if (inside > 0) {
-            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]),
-                           "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
-                         : "l"(reinterpret_cast<const uint32_t*>(p) + i));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[i + j] = 0;
-          }
+      for (int i = 0; i < N * (int)sizeof(T) / 4; i += kVec / 4) {
+        if constexpr (kVec == 32) {
+          asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                       : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]),
+                         "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                       : "l"(q + i));
+        } else if constexpr (kVec == 16) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q + i);
+          w[i] = x.x;
+          w[i + 1] = x.y;
+          w[i + 2] = x.z;
+          w[i + 3] = x.w;
+        } else if constexpr (kVec == 8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(q + i);
+          w[i] = x.x;
+          w[i + 1] = x.y;
+        } else {
+          w[i] = q[i];
         }
-      } else if constexpr (kBytes >= 16) {
-#pragma unroll
-        for (int i = 0; i < kBytes / 16; ++i)
-          reinterpret_cast<uint4*>(v)[i] =
-              inside > 0 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
-      } else if constexpr (kBytes == 8) {
-        *reinterpret_cast<uint2*>(v) =
-            inside > 0 ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
-      } else {
-        *reinterpret_cast<uint32_t*>(v) = inside > 0 ? *reinterpret_cast<const uint32_t*>(p) : 0u;
       }
       return;
     }
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = j < inside ? p[j] : T();
+  for (int j = 0; j < N; ++j) v[j] = j < at.n ? row[at.e0 + j] : T();
 }
 
 template <int N, typename T>
-__device__ __forceinline__ void store_n(T* p, bool wide, int inside, const T (&v)[N]) {
-  constexpr int kBytes = N * (int)sizeof(T);
-  if constexpr (kBytes >= 4) {
+__device__ __forceinline__ void store_n(T* p, bool wide, int n, const T (&v)[N]) {
+  constexpr int kVec = vector_bytes(N * (int)sizeof(T));
+  if constexpr (kVec > 0) {
     if (wide) {
-      if (inside <= 0) return;
-      if constexpr (kBytes >= 32) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+      if (n <= 0) return;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+      uint32_t* q = reinterpret_cast<uint32_t*>(p);
 #pragma unroll
-        for (int i = 0; i < kBytes / 4; i += 8) {
+      for (int i = 0; i < N * (int)sizeof(T) / 4; i += kVec / 4) {
+        if constexpr (kVec == 32) {
           const uint32_t x[8] = {w[i],     w[i + 1], w[i + 2], w[i + 3],
                                  w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
-          sm100::st_global_v8(reinterpret_cast<uint32_t*>(p) + i, x);
+          sm100::st_global_v8(q + i, x);
+        } else if constexpr (kVec == 16) {
+          *reinterpret_cast<uint4*>(q + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else if constexpr (kVec == 8) {
+          *reinterpret_cast<uint2*>(q + i) = make_uint2(w[i], w[i + 1]);
+        } else {
+          q[i] = w[i];
         }
-      } else if constexpr (kBytes >= 16) {
-#pragma unroll
-        for (int i = 0; i < kBytes / 16; ++i)
-          reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
-      } else if constexpr (kBytes == 8) {
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
-      } else {
-        *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(v);
       }
       return;
     }
   }
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    if (j < inside) p[j] = v[j];
+    if (j < n) p[j] = v[j];
 }
 
-// The lane's logits; experts past E and unusable ones (NaN) become -inf.
+// The lane's logits; experts that are not there and unusable ones (NaN) become -inf.
 template <int EPL, typename In>
-__device__ __forceinline__ void load_logits(const RouterArgs& a, int64_t t, int lane,
+__device__ __forceinline__ void load_logits(const RouterArgs& a, int64_t t, const Place& at,
                                             float (&x)[EPL]) {
-  const int e0 = lane * EPL;
   alignas(16) In raw[EPL];
-  load_n(static_cast<const In*>(a.logits) + t * a.stride + e0, a.wide, a.E - e0, raw);
+  load_n(static_cast<const In*>(a.logits) + t * a.stride, at, a.wide, raw);
   // (NaN is the smaller of the two to fmaxf)
 #pragma unroll
   for (int j = 0; j < EPL; ++j) x[j] = fmaxf(to_float(raw[j]), neg_inf());
   if (a.E < EPL * 32) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j)
-      if (e0 + j >= a.E) x[j] = neg_inf();
+      if (j >= at.n) x[j] = neg_inf();
   }
 }
 
@@ -221,16 +237,16 @@ __device__ __forceinline__ void warp_best(double& v, int& e) {
 }
 
 template <int EPL>
-__device__ __forceinline__ void load_bias_n(const RouterArgs& a, int lane, float (&b)[EPL]) {
-  const int e0 = lane * EPL;
+__device__ __forceinline__ void load_bias_n(const RouterArgs& a, const Place& at,
+                                            float (&b)[EPL]) {
   if (a.bias_bf16) {
     alignas(16) __nv_bfloat16 raw[EPL];
-    load_n(static_cast<const __nv_bfloat16*>(a.bias) + e0, a.wide, a.E - e0, raw);
+    load_n(static_cast<const __nv_bfloat16*>(a.bias), at, a.wide, raw);
 #pragma unroll
     for (int j = 0; j < EPL; ++j) b[j] = __bfloat162float(raw[j]);
   } else {
     alignas(16) float raw[EPL];
-    load_n(static_cast<const float*>(a.bias) + e0, a.wide, a.E - e0, raw);
+    load_n(static_cast<const float*>(a.bias), at, a.wide, raw);
 #pragma unroll
     for (int j = 0; j < EPL; ++j) b[j] = raw[j];
   }
@@ -265,10 +281,53 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
   return r;
 }
 
-// An expert's biased sigmoid score in 64 bits. Not inlined: tokens that need it are rare, and
-// their warp waits for the code.
+// An expert's biased sigmoid score, and its share of a softmax before the division, in 64 bits.
+// Not inlined: tokens that need them are rare, and their warp waits for the code.
 __device__ __noinline__ double exact_score(float x, float bias) {
   return 1.0 / (1.0 + exp(-(double)x)) + (double)bias;
+}
+
+__device__ __noinline__ double exact_share(float x, float top) {
+  return exp((double)x - (double)top);
+}
+
+// Whether the lane's group is one of the best by the sum of its two best scores, found from the
+// keys of its two best 16-bit logits (0: none); -1 where a softmax needs its whole row. Not
+// inlined: as part of its caller it cost the routers that do not come here 2 %.
+template <typename In>
+__device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, bool softmax,
+                                       int n_group, int topk_group, int span_log2, int lane) {
+  const float kLog2e = 1.4426950408889634f;
+  const int own = lane >> span_log2;
+  const float x1 = b1 ? to_float(row[0xffffu - (b1 & 0xffffu)]) : neg_inf();
+  const float x2 = b2 ? to_float(row[0xffffu - (b2 & 0xffffu)]) : neg_inf();
+  const float top = warp_max(x1);
+  if (softmax && !(fabsf(top) < 1e30f)) return -1;  // an infinity, or no expert at all
+  auto score = [&](float x) {
+    return softmax ? fast_exp2((x - top) * kLog2e)
+                   : fast_reciprocal(1.0f + fast_exp2(x * -kLog2e));
+  };
+  // below all others: too few usable experts; such groups are told apart by their index
+  const float mine = b2 ? score(x1) + score(x2) : -1.0f;
+  int rank = 0;
+  for (int h = 0; h < n_group; ++h) {
+    const float v = __shfl_sync(kAll, mine, h << span_log2);
+    rank += v > mine || (v == mine && h < own);
+  }
+  bool keep = rank < topk_group;
+  const float worst = warp_min(keep ? mine : 4.0f), best = warp_max(keep ? -1.0f : mine);
+  if (best >= 0.0f && worst - best <= 16 * 0x1p-23f) {  // a score's error is 8 * 2^-24
+    const double sum = !b2       ? -1.0
+                       : softmax ? exact_share(x1, top) + exact_share(x2, top)
+                                 : exact_score(x1, 0.0f) + exact_score(x2, 0.0f);
+    rank = 0;
+    for (int h = 0; h < n_group; ++h) {
+      const double v = __shfl_sync(kAll, sum, h << span_log2);
+      rank += v > sum || (v == sum && h < own);
+    }
+    keep = rank < topk_group;
+  }
+  return keep;
 }
 
 // Picks by one 32-bit key an expert: its value in the high bits, its index (reversed, so that
@@ -279,20 +338,23 @@ __device__ __noinline__ double exact_score(float x, float bias) {
 //            roundings). Where two sigmoid scores that matter are not told apart, those alone are
 //            taken in 64 bits; where that does not do (a softmax needs its whole row; the
 //            runner-up is near too) the result is false.
-//   no bias  16-bit logits as they are: exact
+//   no bias  16-bit logits as they are: exact; a group's two best scores follow from its two best
+//            logits, in 64 bits where two groups are not told apart
 // Groups are whole runs of lanes, or there are none.
 template <int EPL, typename In>
 __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
-                                              const float (&x)[EPL], int lane, int& pick) {
-  constexpr int kScoreBits = EPL <= 8 ? 8 : EPL == 16 ? 9 : 10;  // index bits beside a score
-  const int e0 = lane * EPL;
+                                              const float (&x)[EPL], const Place& place, int lane,
+                                              int& pick) {
+  constexpr int kScoreBits = EPL <= 8 ? 8 : EPL <= 16 ? 9 : 10;  // index bits beside a score
+  const float kLog2e = 1.4426950408889634f;
+  const int e0 = place.e0;
   uint32_t p[EPL];
   const int bits = a.bias ? kScoreBits : 16;
   uint32_t near = 0;  // values that differ by no more are not told apart
   if (a.bias) {
-    const float kNaN = __int_as_float(0x7fffffff), kLog2e = 1.4426950408889634f;
+    const float kNaN = __int_as_float(0x7fffffff);
     float c[EPL], b[EPL];
-    load_bias_n<EPL>(a, lane, b);
+    load_bias_n<EPL>(a, place, b);
     float tol;
     // experts that may not be used become NaN, which minima and maxima pass over
     if (a.softmax) {
@@ -376,7 +438,22 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
     return exact_score(to_float(static_cast<const In*>(a.logits)[t * a.stride + e]),
                        load_bias(a, e));
   };
-  if (a.n_group > 1) {
+  if (a.n_group > 1 && !a.bias && !a.group_max) {
+    const int span = 1 << a.span_log2;
+    uint32_t b1 = p[0], b2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] : 0u;
+    for (int o = 1; o < span; o <<= 1) {
+      const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
+      b2 = max(min(b1, q1), max(b2, q2));
+      b1 = max(b1, q1);
+    }
+    const int keep = keep_group(static_cast<const In*>(a.logits) + t * a.stride, b1, b2,
+                                a.softmax, a.n_group, a.topk_group, a.span_log2, lane);
+    if (keep < 0) return false;
+    if (!keep) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) p[j] = 0u;
+    }
+  } else if (a.n_group > 1) {
     const int span = 1 << a.span_log2, own = lane >> a.span_log2;
     uint32_t m1 = p[0] >> bits, m2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] >> bits : 0u;
     for (int o = 1; o < span; o <<= 1) {
@@ -413,7 +490,8 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
           b1 = max(b1, q1);
         }
         const uint32_t last = a.group_max ? b1 : b2, after = a.group_max ? b2 : b3;
-        if (__any_sync(kAll, last && after && (last >> bits) - (after >> bits) <= near)) return false;
+        if (__any_sync(kAll, last && after && (last >> bits) - (after >> bits) <= near))
+          return false;
         double score = (double)neg_inf();
         if (last) {
           score = exact((int)(mask - (b1 & mask)));
@@ -482,10 +560,10 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
 // follow the logits, which need no arithmetic.
 template <int EPL, typename V>
 __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float (&x)[EPL],
-                                               int lane, int& pick) {
+                                               const Place& place, int lane, int& pick) {
   constexpr bool kFast = sizeof(V) == 4;
   const V kNone = (V)neg_inf();
-  const int e0 = lane * EPL;
+  const int e0 = place.e0;
   const bool by_group = a.n_group > 1;
   const bool scored = a.bias || (by_group && !a.group_max);
   V worth[EPL], c[EPL];
@@ -518,7 +596,7 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
     float far = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      if (e0 + j >= a.E) continue;
+      if (j >= place.n) continue;
       const float b = load_bias(a, e0 + j);
       worth[j] += (V)b;
       if (kFast && b > neg_inf()) far = fmaxf(far, fabsf(b));
@@ -536,10 +614,9 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
     V mine = kNone;  // the score of the lane's group: lane g's, or lane / span's
     int own = lane, span = 1;
     // groups of whole lanes: the lanes of a group merge their two best
-    const bool whole = EPL * 32 == a.E && 32 % a.n_group == 0;
-    if (whole) {
-      span = 32 / a.n_group;
-      own = lane / span;
+    if (a.whole) {
+      span = 1 << a.span_log2;
+      own = lane >> a.span_log2;
       V m1 = kNone, m2 = kNone;
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
@@ -591,12 +668,12 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
         if (own < a.n_group && other && !(fabsf((float)(v - mine)) > 2.0f * tol)) sure = false;
       }
     }
-    if (whole) {
+    if (a.whole) {
       if (!((votes >> lane) & 1u)) live = 0;
     } else {
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
-        if (e0 + j < a.E && !((votes >> ((e0 + j) / G)) & 1u)) live &= ~(1u << j);
+        if (j < place.n && !((votes >> ((e0 + j) / G)) & 1u)) live &= ~(1u << j);
     }
   }
   pick = -1;
@@ -616,7 +693,7 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
     if (compare && k > 0 && !((float)(last - best) > tol)) sure = false;
     last = best;
     if (k == a.K) break;
-    if (at / EPL == lane) live &= ~(1u << (at % EPL));
+    if ((uint32_t)(at - e0) < (uint32_t)EPL) live &= ~(1u << (at - e0));
     if (lane == k) pick = at;
   }
   return !kFast || __all_sync(kAll, sure);
@@ -650,26 +727,33 @@ __device__ __forceinline__ void row_softmax(const float (&x)[EPL], float& top, f
   sum = warp_sum(sum);
 }
 
+// Resident blocks an SM: issue-bound, so warps count for more than the registers that the rare
+// 64-bit paths lack. 16384 x 256: 16.2 us with 4, 17.3 with 3; 16384 x 384: 21 us with 3, 45
+// with 1.
+constexpr int router_blocks(int epl) { return epl <= 4 ? 5 : epl <= 8 ? 4 : epl <= 16 ? 3 : 2; }
+
 template <int EPL, typename In>
-__global__ void __launch_bounds__(kRouterWarps * 32, EPL <= 8 ? 4 : 1) route_experts_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(kRouterWarps * 32, router_blocks(EPL))
+    route_experts_kernel(RouterArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
   if (t >= a.T) return;
+  const Place place = place_of<EPL>(a, lane);
   float x[EPL];
-  load_logits<EPL, In>(a, t, lane, x);
+  load_logits<EPL, In>(a, t, place, x);
   int pick;
-  bool sure = false;
-  if (a.by_key && (a.bias || sizeof(In) == 2)) sure = select_by_key<EPL, In>(a, t, x, lane, pick);
-  else sure = select_experts<EPL, float>(a, x, lane, pick);
-  if (!sure) select_experts<EPL, double>(a, x, lane, pick);
+  bool sure;
+  if (a.by_key && (a.bias || sizeof(In) == 2))
+    sure = select_by_key<EPL, In>(a, t, x, place, lane, pick);
+  else
+    sure = select_experts<EPL, float>(a, x, place, lane, pick);
+  if (!sure) select_experts<EPL, double>(a, x, place, lane, pick);
   float top = 0.0f, sum = 1.0f;
   if (a.softmax && !a.renorm) row_softmax<EPL>(x, top, sum);
   const float xp =
       pick >= 0 ? to_float(static_cast<const In*>(a.logits)[t * a.stride + pick]) : 0.0f;
   float w = pick_weight(a, pick, xp, top, sum);
-  if (a.renorm && !a.softmax) {
-    w *= __frcp_rn(warp_sum(w) + 1e-20f);
-  }
+  if (a.renorm && !a.softmax) w *= __frcp_rn(warp_sum(w) + 1e-20f);
   if (lane < a.K) {
     const int64_t at = t * a.K + lane;
     a.idx[at] = pick;
@@ -697,10 +781,11 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(R
   if (!(xp > neg_inf())) pick = -1;
   const float g = pick >= 0 ? a.grad_w[t * a.K + lane] : 0.0f;
   const bool dense = a.softmax && !a.renorm;
+  const Place place = place_of<EPL>(a, lane);
   float x[EPL];
   float top = 0.0f, sum = 1.0f;
   if (dense) {
-    load_logits<EPL, In>(a, t, lane, x);
+    load_logits<EPL, In>(a, t, place, x);
     row_softmax<EPL>(x, top, sum);
   }
   const float s = pick_weight(a, pick, xp, top, sum);
@@ -723,13 +808,12 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(R
   if (pick < 0) d = 0.0f;
   const float all = dense ? warp_sum(d) : 0.0f;
   // every expert's dense part as vectors, then the picks' places again with their own
-  const int e0 = lane * EPL;
   alignas(16) In raw[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j)
     raw[j] = from_float<In>(
         dense && x[j] > neg_inf() ? -all * (exp_below(x[j], top) / sum) : 0.0f);
-  store_n(out + e0, a.wide, a.E - e0, raw);
+  store_n(out + place.e0, a.wide, place.n, raw);
   const unsigned same = __match_any_sync(kAll, pick);
   if (__any_sync(kAll, pick >= 0 && __popc(same) > 1)) {
     // an expert named several times: its first pick takes the terms of all
@@ -799,23 +883,21 @@ RouterArgs router_args(const fmoe_router* r, const void* logits) {
 }
 
 // Whether a lane's N values of every row, of the bias and of a gradient row are aligned vectors
-// that lie inside the row or outside of it.
+// that are there all or not at all.
 template <int N, typename In>
 bool vectors(const RouterArgs& a) {
-  const size_t bytes = N * sizeof(In) < 32 ? N * sizeof(In) : 32;
-  const size_t bias = a.bias_bf16 ? 2 : 4;
-  const size_t bias_bytes = N * bias < 32 ? N * bias : 32;
-  return a.E % N == 0 && a.stride % N == 0 && bytes >= 4 && bias_bytes >= 4 &&
+  const int bytes = vector_bytes(N * (int)sizeof(In));
+  const int bias = vector_bytes(N * (a.bias_bf16 ? 2 : 4));
+  if (a.run % N != 0 || bytes == 0 || (a.bias && bias == 0)) return false;
+  return a.stride * (int64_t)sizeof(In) % bytes == 0 &&
          reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
          reinterpret_cast<uintptr_t>(a.grad_logits) % bytes == 0 &&
-         reinterpret_cast<uintptr_t>(a.bias) % bias_bytes == 0;
+         (!a.bias || reinterpret_cast<uintptr_t>(a.bias) % bias == 0);
 }
 
 template <int EPL, typename In>
 void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
   a.wide = vectors<EPL, In>(a);
-  while ((32 >> a.span_log2) > a.n_group) ++a.span_log2;
-  a.by_key = a.n_group == 1 || (EPL * 32 == a.E && 32 % a.n_group == 0 && (a.bias || a.group_max));
   const unsigned grid = (unsigned)((a.T + kRouterWarps - 1) / kRouterWarps);
   if (backward)
     route_experts_grad_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
@@ -824,12 +906,26 @@ void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
 }
 
 template <typename In>
-void launch_router(const RouterArgs& a, bool backward, cudaStream_t stream) {
-  if (a.E <= 32) launch_router<1, In>(a, backward, stream);
-  else if (a.E <= 64) launch_router<2, In>(a, backward, stream);
-  else if (a.E <= 128) launch_router<4, In>(a, backward, stream);
-  else if (a.E <= 256) launch_router<8, In>(a, backward, stream);
-  else if (a.E <= 512) launch_router<16, In>(a, backward, stream);
+void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
+  // a run of experts for 32 / n_group lanes where that is whole, else all for all lanes
+  a.span_log2 = 5;
+  a.run = a.E;
+  a.whole = a.n_group > 1 && (a.n_group & (a.n_group - 1)) == 0;
+  if (a.whole) {
+    while ((32 >> a.span_log2) < a.n_group) --a.span_log2;
+    a.run = a.E / a.n_group;
+  }
+  a.by_key = a.whole || a.n_group == 1;
+  const int lanes = 1 << a.span_log2, need = (a.run + lanes - 1) / lanes;
+  if (need <= 1) launch_router<1, In>(a, backward, stream);
+  else if (need <= 2) launch_router<2, In>(a, backward, stream);
+  else if (need <= 3) launch_router<3, In>(a, backward, stream);
+  else if (need <= 4) launch_router<4, In>(a, backward, stream);
+  else if (need <= 5) launch_router<5, In>(a, backward, stream);
+  else if (need <= 6) launch_router<6, In>(a, backward, stream);
+  else if (need <= 8) launch_router<8, In>(a, backward, stream);
+  else if (need <= 12) launch_router<12, In>(a, backward, stream);
+  else if (need <= 16) launch_router<16, In>(a, backward, stream);
   else launch_router<32, In>(a, backward, stream);
 }
 

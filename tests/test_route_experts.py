@@ -49,7 +49,8 @@ RULES = [
     (1, 1, 1, 1, "top2"), (8, 2, 1, 1, "max"), (16, 4, 4, 2, "top2"), (72, 8, 3, 1, "max"),
     (160, 6, 8, 3, "max"), (512, 16, 32, 7, "top2"), (1000, 32, 4, 2, "top2"), (33, 32, 1, 1, "max"),
     (64, 6, 2, 1, "top2"), (128, 8, 4, 2, "max"), (32, 4, 16, 5, "max"), (512, 8, 2, 1, "max"),
-    (1024, 8, 4, 3, "top2"),
+    (1024, 8, 4, 3, "top2"), (384, 15, 2, 1, "top2"), (96, 7, 4, 3, "top2"), (72, 4, 8, 6, "max"),
+    (40, 4, 8, 2, "top2"), (640, 8, 4, 2, "top2"), (384, 8, 1, 1, "max"), (66, 5, 2, 2, "top2"),
 ]
 
 
@@ -147,6 +148,27 @@ def test_route_experts_crowded_scores(fmoe, score, E, K, n, kg, how):
                                     group_score=how, bias=None if bias is None else bias.cuda())
         want, _ = ref.route(logits, bias, K, score, n, kg, how)
         assert torch.equal(idx.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,K,n,kg", [(256, 8, 8, 4), (160, 6, 8, 3), (64, 6, 2, 1), (32, 4, 16, 5),
+                                      (60, 6, 6, 2)])
+def test_route_experts_groups_without_bias(fmoe, score, dtype, E, K, n, kg):
+    """Groups whose two best scores tie, or differ by less than single precision resolves (large
+    negative logits), or of which one or none may be used."""
+    g = torch.Generator().manual_seed(E + n)
+    x = torch.randint(-6, 7, (80, E), generator=g) / 2 + 0.125
+    x[20:40] -= 40
+    x[40:60] = 9 + torch.randint(0, 8, (20, E), generator=g) / 16  # sigmoids close to 1
+    x[60:] = x[60:].masked_fill(torch.rand(20, E, generator=g) < 0.9, -math.inf)
+    x[79] = -math.inf
+    x = x.to(dtype)
+    idx, w = fmoe.route_experts(x.cuda(), K, score=score, n_group=n, topk_group=kg)
+    want_idx, want_w = ref.route(x, None, K, score, n, kg, "top2")
+    assert torch.equal(idx.cpu(), want_idx)
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
 
 
 @pytest.mark.gpu
