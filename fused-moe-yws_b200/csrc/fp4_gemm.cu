@@ -363,11 +363,10 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 
-// kSplit > 1 (few rows, so fewer tiles than would keep every SM reading): in the last round of
-// tiles the CTAs of a cluster share a tile of at most 32 rows, each a part of the K steps. CTA r
-// finishes the tile's slice r of the columns (swiglu: of the features): the others store their
-// sums of that slice into its shared memory, it adds them in the order of the ranks. A tile of
-// more rows is the first CTA's, whole.
+// kSplit > 1 (at most 32 rows, so fewer tiles than would keep every SM reading): the CTAs of a
+// cluster share one tile, each a part of the K steps. CTA r finishes the tile's slice r of the
+// columns: the others store their sums of that slice into its shared memory, it adds them in the
+// order of the ranks. 16 x 4096 x 7168: 8.9 us, 15 with whole tiles.
 template <int kFormat, int BN, Epilogue kEpi, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
@@ -390,7 +389,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 22);
   int* err = reinterpret_cast<int*>(bars + 23);
   uint64_t* xfull = bars + 24;   // the other CTAs' sums of this one's slice have come
-  uint64_t* xfree = bars + 25;   // the other CTAs have read this one's
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -403,10 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tempty[b], kEpiWarps);
     }
     mbar_init(mma_done, 1);
-    if (kSplit > 1) {
-      mbar_init(xfull, 32 * (kSplit - 1));
-      mbar_init(xfree, 32 * (kSplit - 1));
-    }
+    if (kSplit > 1) mbar_init(xfull, 32 * (kSplit - 1));
     *abort_flag = 0;
     *err = 0;
     fence_mbar_init();
@@ -445,30 +440,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int steps = (p.K + kStepCols - 1) / kStepCols;
   const int across = tiles_across(p.K, kFormat);  // scale tiles per 128 rows
   const uint32_t rank = kSplit > 1 ? cluster_rank() : 0;
-  // Tiles [0, whole) go round-robin to the CTAs, those behind them to the clusters: the last
-  // round where it would leave half of the CTAs without a tile.
-  const int64_t total = (int64_t)(p.experts ? s_first[p.experts] : p.m_tiles) * p.n_tiles;
-  const int64_t G = gridDim.x, clusters = G / kSplit;
-  int64_t whole = total;
-  if (kSplit > 1 && total % G <= clusters) whole = total - total % G;
-  const int64_t mine_whole = (whole - blockIdx.x + G - 1) / G;
-  // Tile j of this CTA and its K steps [k0, k1); false: no more. K steps none: not its part.
-  auto next = [&](int64_t j, Tile& t, int& k0, int& k1, bool& shared) {
-    k0 = 0;
-    k1 = steps;
-    shared = false;
-    if (j < mine_whole) return tile_of(p, s_first, s_count, blockIdx.x + j * G, t);
-    if (kSplit == 1) return false;
-    const int64_t i = whole + blockIdx.x / kSplit + (j - mine_whole) * clusters;
-    if (!tile_of(p, s_first, s_count, i, t)) return false;
-    shared = t.rows <= 32;
-    if (shared) {
-      k0 = steps * (int)rank / kSplit;
-      k1 = steps * ((int)rank + 1) / kSplit;
-    } else if (rank != 0) {
-      k1 = 0;
-    }
-    return true;
+  // the tile's K steps [k0, k1) of this CTA
+  const int k0 = steps * (int)rank / kSplit, k1 = steps * ((int)rank + 1) / kSplit;
+  // Tile j of this CTA (round-robin; a cluster has one); false: no more.
+  auto next = [&](int64_t j, Tile& t) {
+    if (kSplit > 1) return j == 0 && tile_of(p, s_first, s_count, blockIdx.x / kSplit, t);
+    return tile_of(p, s_first, s_count, blockIdx.x + j * gridDim.x, t);
   };
   // how many tiles back the accumulator of a tile must have been read
   constexpr int kBack = C::kOverlapped ? 1 : 2;
@@ -480,10 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       bool ok = true;
       Tile t;
-      int k0, k1;
-      bool shared;
-      for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
-        if (k1 == 0) continue;
+      for (int64_t j = 0; ok && next(j, t); ++j) {
         // the 128-row runs of b: next to each other, or gate and up rows
         int row[C::kRuns], runs = 0;
         const uint8_t* sb[C::kRuns];
@@ -533,10 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0;
       bool ok = true;
       Tile t;
-      int k0, k1;
-      bool shared;
-      for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
-        if (k1 == 0) continue;
+      for (int64_t j = 0; ok && next(j, t); ++j) {
         const uint8_t* sa = p.sa + (int64_t)t.m * across * kTileBytes;
         // few rows: boxes of 32 (the other rows of the stage keep what they held; a row of a
         // only reaches its own row of the product)
@@ -574,10 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Tile t;
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t st0 = __shfl_sync(0xffffffffu, smem_addr(stages), 0);
-    int k0, k1;
-    bool shared;
-    for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
-      if (k1 == 0) continue;
+    for (int64_t j = 0; ok && next(j, t); ++j) {
       if (n >= kBack &&
           !mbar_wait(&tempty[(n - kBack) & 1], ((n - kBack) >> 1) & 1, abort_flag))
         ok = false;
@@ -640,11 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int n = 0;
     bool ok = true;
     Tile t;
-    uint32_t shared_tiles = 0;  // tiles that the cluster shared so far
-    int k0, k1;
-    bool shared;
-    for (int64_t j = 0; ok && next(j, t, k0, k1, shared); ++j) {
-      if (k1 == 0) continue;
+    for (int64_t j = 0; ok && next(j, t); ++j) {
       const int row = q * 32 + lane;
       const int64_t m = (int64_t)t.m * 128 + row, m0 = m - lane;
       const int rows = t.rows - q * 32;  // of this warp's 32
@@ -657,22 +621,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1) * C::kAcc1 + ((uint32_t)(q * 32) << 16);
       const int n0 = t.n * BN;
-      if (kSplit > 1 && shared) {
+      if constexpr (kSplit > 1) {
         // ---- a tile that the cluster shares: rows 0..31, so only the warps of lanes 0..31
-        constexpr int V = C::kSlice, F = V / 2;  // F: features of a slice (swiglu)
-        auto column = [](int s, int c) {         // the first column of a slice's chunk c of 32
-          if (kEpi != kSwiglu) return s * V + 32 * c;
-          return c < F / 32 ? s * F + 32 * c : 128 + s * F + 32 * (c - F / 32);
-        };
+        static_assert(kEpi == kStore && !C::kOverlapped, "a cluster's tile");
+        constexpr int V = C::kSlice;
         const bool mine = q == 0 && (int)rank / (kSplit / 2) == half;
-        // (only warps that send wait for the slot: the others could fall two phases behind)
         if (q == 0 && (kSplit > 2 || !mine)) {
-          if (shared_tiles > 0 && !mbar_wait_cluster(xfree, (shared_tiles - 1) & 1, abort_flag))
-            ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
 #pragma unroll
           for (int j = 0; j < kSplit / 2; ++j) {
             const int s = half * (kSplit / 2) + j;
@@ -683,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < V / 32; ++c) {
               uint32_t v[32];
-              tmem_ld_32x32b<32>(acc + column(s, c), v);
+              tmem_ld_32x32b<32>(acc + s * V + 32 * c, v);
               tmem_ld_wait();
 #pragma unroll
               for (int x = 0; x < 8; ++x)
@@ -694,14 +648,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (mine) {
-          if (!mbar_wait_cluster(xfull, shared_tiles & 1, abort_flag)) ok = false;
+          if (!mbar_wait_cluster(xfull, 0, abort_flag)) ok = false;
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
-          // chunk c of this CTA's slice: the ranks' parts added in their order
-          auto total = [&](int c, uint32_t (&v)[32]) {
-            tmem_ld_32x32b<32>(acc + column((int)rank, c), v);
+          // the slice: the ranks' parts added in their order
+#pragma unroll
+          for (int c = 0; c < V / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b<32>(acc + (int)rank * V + 32 * c, v);
             tmem_ld_wait();
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
@@ -725,45 +681,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int y = 0; y < 4; ++y) v[4 * x + y] = __float_as_uint(sum[y]);
             }
-          };
-          if constexpr (kEpi == kSwiglu) {
-            const int I = p.N / 2, c0 = t.n * 128 + (int)rank * F;
-            uint32_t bytes = 0;
-#pragma unroll
-            for (int h = 0; h < F / 32; ++h) {
-              uint32_t gate[32], up[32];
-              total(h, gate);
-              total(F / 32 + h, up);
-              uint4 codes;
-              const uint32_t b = swiglu32<kFormat>(gate, up, alpha, divisor, codes);
-              bytes |= b << (kFormat == FMOE_MXFP4 ? 8 * h : 16 * h);
-              if (row < t.rows)
-                *reinterpret_cast<uint4*>(p.codes + m * (I / 2) + c0 / 2 + 16 * h) = codes;
-            }
-            if (row < t.rows) {
-              const int block = c0 / block_of(kFormat);
-              uint8_t* sc = p.scales +
-                            ((int64_t)t.m * tiles_across(I, kFormat) + block / 4) * kTileBytes +
-                            scale_offset(row, block);
-              if (kFormat == FMOE_MXFP4) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)bytes;
-              else *reinterpret_cast<uint32_t*>(sc) = bytes;
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < V / 32; ++c) {
-              uint32_t v[32];
-              total(c, v);
-              store32(p, m0, rows, n0 + column((int)rank, c), v, alpha, wide);
-            }
+            store32(p, m0, rows, n0 + (int)rank * V + 32 * c, v, alpha, wide);
           }
-#pragma unroll
-          for (int r = 0; r < kSplit; ++r)
-            if (r != (int)rank) peer_arrive(peer_addr(smem_addr(xfree), r));
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[n & 1]);
-        ++shared_tiles;
       } else if constexpr (kEpi == kSwiglu) {
         // this warp's 64 gate columns (col) and 64 up columns (128 + col). The side that lies in
         // the columns shared with the next tile comes first: up in the first accumulator
@@ -905,9 +825,7 @@ cudaError_t launch(const Maps& maps, const GemmFp4Args& p, int clusters, cudaStr
 template <int kFormat>
 cudaError_t launch(int bn, int split, bool swiglu, const Maps& maps, const GemmFp4Args& p,
                    int clusters, cudaStream_t stream) {
-  if (swiglu && split > 1) return launch<kFormat, 256, kSwiglu, 2>(maps, p, clusters, stream);
   if (swiglu) return launch<kFormat, 256, kSwiglu, 1>(maps, p, clusters, stream);
-  if (bn == 256 && split > 1) return launch<kFormat, 256, kStore, 2>(maps, p, clusters, stream);
   if (bn == 256) return launch<kFormat, 256, kStore, 1>(maps, p, clusters, stream);
   if (split == 4) return launch<kFormat, 128, kStore, 4>(maps, p, clusters, stream);
   if (split == 2) return launch<kFormat, 128, kStore, 2>(maps, p, clusters, stream);
@@ -954,7 +872,8 @@ int launch_fp4_gemm(const Fp4Gemm& g, cudaStream_t stream) {
       return ((int64_t)p.m_tiles * ((g.N + n - 1) / n) + sms - 1) / sms;
     };
     if (rounds(128) * 36 <= rounds(256) * 54) bn = 128;
-    // few rows and too few tiles: tiles shared by 2 or 4 CTAs, as long as each has two K steps
+    // few rows and too few tiles: tiles shared by 2 or 4 CTAs, as long as each has two K steps;
+    // at most one tile a cluster
     if (g.M <= 32 && bn == 128) {
       const int tiles = (g.N + bn - 1) / bn;
       while (split < 4 && tiles * split * 2 <= sms && steps >= 4 * split) split *= 2;
