@@ -188,8 +188,8 @@ bool fused(const fmoe_fp4_problem* p) { return p->intermediate_size % 128 == 0; 
 // The expert's rows in fp32, where they fit the cache between the product that writes them and
 // the sum that reads them: the result is rounded once. Larger batches round each row to bf16
 // too, which with k rows a token adds as much error again (2.4e-3 for 1.7e-3, of the plain
-// product in fp32), but halves 0.9 GB of traffic for 4096 tokens with 8 local picks each (H
-// 7168): 147 us at the memory's rate, next to about 1.2 ms of products.
+// product in fp32), but halves 0.9 GB of rows each way for 4096 tokens with 8 local picks each (H
+// 7168, 32 experts): 986 us, 1158 with fp32 rows. At 16 and 256 tokens the two take as long.
 bool exact_rows(const fmoe_fp4_problem* p) {
   return p->num_tokens * p->top_k * p->hidden_size * 4 <= (int64_t)64 << 20;
 }
