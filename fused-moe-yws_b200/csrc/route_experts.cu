@@ -510,27 +510,33 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
       for (int j = 0; j < EPL; ++j) p[j] = 0u;
     }
   }
-  uint32_t gap = 0xffffffffu, last = 0xffffffffu, won = 0;  // gap: of neighbours in the order
+  // one round more than there are picks where a near runner-up matters; past the last usable
+  // expert a round finds 0
+  uint32_t last = 0, won = 0;
   const int rounds = a.K + (near ? 1 : 0);
-  int found = 0;
-#pragma unroll 2
-  for (; found < rounds; ++found) {
-    const uint32_t top = __reduce_max_sync(kAll, p[0]);
-    if (top == 0) break;  // fewer usable experts than top_k
-    gap = min(gap, last - top);
-    last = top;
-    if (lane == found) won = top;
-    const bool mine = p[0] == top;
+#pragma unroll 4
+  for (int k = 0; k < rounds; ++k) {
+    last = __reduce_max_sync(kAll, p[0]);
+    if (lane == k) won = last;
+    const bool mine = p[0] == last;
 #pragma unroll
     for (int j = 0; j + 1 < EPL; ++j) p[j] = mine ? p[j + 1] : p[j];
     p[EPL - 1] = mine ? 0u : p[EPL - 1];
   }
   pick = won ? (int)(mask - (won & mask)) : -1;
+  uint32_t gap = 0xffffffffu;  // the smallest of neighbours in the order
+  if (near) {
+    const uint32_t before = __shfl_up_sync(kAll, won, 1);
+    if (lane > 0 && won) gap = before - won;
+    if (rounds > 32 && lane == 31 && last) gap = min(gap, won - last);
+    gap = __reduce_min_sync(kAll, gap);
+  }
   if (near && (gap >> bits) <= near) {
+    const int found = __popc(__ballot_sync(kAll, won != 0));
     // the picks and the runner-up in 64 bits, put in order by counting; the one behind them has to
     // be clear of them
     const uint32_t behind = __reduce_max_sync(kAll, p[0]);
-    if (a.softmax || found > 32 || (behind && (last >> bits) - (behind >> bits) <= near))
+    if (a.softmax || rounds > 32 || (behind && (last >> bits) - (behind >> bits) <= near))
       return false;
     const double score = pick >= 0 ? exact(pick) : 0.0;
     int rank = 0;
