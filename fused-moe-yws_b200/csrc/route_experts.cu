@@ -15,11 +15,10 @@
 // One warp routes one token, a lane holds up to EPL consecutive experts; where the number of
 // groups is a power of two, 32 / n_group lanes hold a group's (Place), so that groups of any size
 // merge by shuffles: 14932 x 160 in 8 groups takes 11 us, 55 where a lane's experts cross groups;
-// with 16384 x 256 the mapping costs 0.5 us of 16. Small batches are
-// bound by the latency of a warp's chain (3.2 us for one token, launch included), large ones by
-// instruction issue: 16384 x 256 with bias and groups runs 750 instructions a token in 16.5 us,
-// where reading the logits takes 2.6 us. All in 64 bits it took 104 us, with compared (value,
-// index) pairs in place of select_by_key's keys 40 us.
+// with 16384 x 256 the mapping costs 0.5 us of 16. Small batches are bound by the latency of a
+// warp's chain (3.2 us for one token, launch included), large ones by instruction issue:
+// 16384 x 256 with bias and groups takes 15.5 us, where reading the logits takes 2.6 us. All in
+// 64 bits it took 104 us, with compared (value, index) pairs in place of select_by_key's keys 40.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,7 +35,10 @@
 namespace fmoe {
 namespace {
 
-constexpr int kRouterWarps = 8;
+// Tokens (warps) of a block: 16384 x 256 in 15.5 us with 2, 15.9 with 8, 64 x 384 in 3.5 and 3.9;
+// the gradient, which writes whole rows, 6.7 and 6.4.
+constexpr int kRouterWarps = 2;
+constexpr int kGradWarps = 8;
 constexpr int kRouterMaxExperts = 1024;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -733,10 +735,12 @@ __device__ __forceinline__ void row_softmax(const float (&x)[EPL], float& top, f
   sum = warp_sum(sum);
 }
 
-// Resident blocks an SM: issue-bound, so warps count for more than the registers that the rare
-// 64-bit paths lack. 16384 x 256: 16.2 us with 4, 17.3 with 3; 16384 x 384: 21 us with 3, 45
-// with 1.
-constexpr int router_blocks(int epl) { return epl <= 4 ? 5 : epl <= 8 ? 4 : epl <= 16 ? 3 : 2; }
+// Resident warps an SM: issue-bound, so warps count for more than the registers that the rare
+// 64-bit paths lack. 16384 x 256: 16.2 us with 32, 17.3 with 24; 16384 x 384: 21 us with 24, 45
+// with 8.
+constexpr int router_blocks(int epl) {
+  return (epl <= 4 ? 40 : epl <= 8 ? 32 : epl <= 16 ? 24 : 16) / kRouterWarps;
+}
 
 template <int EPL, typename In>
 __global__ void __launch_bounds__(kRouterWarps * 32, router_blocks(EPL))
@@ -775,9 +779,9 @@ __global__ void __launch_bounds__(kRouterWarps * 32, router_blocks(EPL))
 //   sigmoid, plain          d_k = scale g_k s_k (1 - s_k)
 // An expert named by several picks gets the sum of their terms.
 template <int EPL, typename In>
-__global__ void __launch_bounds__(kRouterWarps * 32) route_experts_grad_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(kGradWarps * 32) route_experts_grad_kernel(RouterArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
+  const int64_t t = (int64_t)blockIdx.x * kGradWarps + (threadIdx.x >> 5);
   if (t >= a.T) return;
   const In* row = static_cast<const In*>(a.logits) + t * a.stride;
   In* out = static_cast<In*>(a.grad_logits) + t * a.E;
@@ -904,9 +908,10 @@ bool vectors(const RouterArgs& a) {
 template <int EPL, typename In>
 void launch_router(RouterArgs a, bool backward, cudaStream_t stream) {
   a.wide = vectors<EPL, In>(a);
-  const unsigned grid = (unsigned)((a.T + kRouterWarps - 1) / kRouterWarps);
+  const int warps = backward ? kGradWarps : kRouterWarps;
+  const unsigned grid = (unsigned)((a.T + warps - 1) / warps);
   if (backward)
-    route_experts_grad_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
+    route_experts_grad_kernel<EPL, In><<<grid, kGradWarps * 32, 0, stream>>>(a);
   else
     route_experts_kernel<EPL, In><<<grid, kRouterWarps * 32, 0, stream>>>(a);
 }
