@@ -294,15 +294,16 @@ __device__ __noinline__ double exact_share(float x, float top) {
 }
 
 // Whether the lane's group is one of the best by the sum of its two best scores, found from the
-// keys of its two best 16-bit logits (0: none); -1 where a softmax needs its whole row. Not
-// inlined: as part of its caller it cost the routers that do not come here 2 %.
+// keys of its two best logits (0: none; the index in the bits of `mask`); -1 where a softmax needs
+// its whole row. Not inlined: as part of its caller it cost the routers that do not come here 2 %.
 template <typename In>
-__device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, bool softmax,
-                                       int n_group, int topk_group, int span_log2, int lane) {
+__device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, uint32_t mask,
+                                       bool softmax, int n_group, int topk_group, int span_log2,
+                                       int lane) {
   const float kLog2e = 1.4426950408889634f;
   const int own = lane >> span_log2;
-  const float x1 = b1 ? to_float(row[0xffffu - (b1 & 0xffffu)]) : neg_inf();
-  const float x2 = b2 ? to_float(row[0xffffu - (b2 & 0xffffu)]) : neg_inf();
+  const float x1 = b1 ? to_float(row[mask - (b1 & mask)]) : neg_inf();
+  const float x2 = b2 ? to_float(row[mask - (b2 & mask)]) : neg_inf();
   const float top = warp_max(x1);
   if (softmax && !(fabsf(top) < 1e30f)) return -1;  // an infinity, or no expert at all
   auto score = [&](float x) {
@@ -332,6 +333,16 @@ __device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, 
   return keep;
 }
 
+// The three largest of two lanes' descending triples.
+__device__ __forceinline__ void merge_best(uint32_t& b1, uint32_t& b2, uint32_t& b3, int o) {
+  const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
+  const uint32_t q3 = __shfl_xor_sync(kAll, b3, o);
+  const uint32_t low = min(b1, q1), mid = max(b2, q2);
+  b3 = max(max(min(low, mid), b3), max(q3, min(b2, q2)));
+  b2 = max(low, mid);
+  b1 = max(b1, q1);
+}
+
 // Picks by one 32-bit key an expert: its value in the high bits, its index (reversed, so that
 // the lower index wins a tie) in the low ones. A lane sorts its keys once; a round is one warp
 // maximum and a shift in the winning lane.
@@ -340,8 +351,10 @@ __device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, 
 //            roundings). Where two sigmoid scores that matter are not told apart, those alone are
 //            taken in 64 bits; where that does not do (a softmax needs its whole row; the
 //            runner-up is near too) the result is false.
-//   no bias  16-bit logits as they are: exact; a group's two best scores follow from its two best
-//            logits, in 64 bits where two groups are not told apart
+//   no bias  16-bit logits as they are: exact. Of 32-bit ones the key holds the upper 22 to 24
+//            bits, and where two that matter have the same the logits themselves decide. A group's
+//            two best scores follow from its two best logits, in 64 bits where two groups are not
+//            told apart. (21794 x 128 in 13.6 us; by compared (value, index) pairs 31.)
 // Groups are whole runs of lanes, or there are none.
 template <int EPL, typename In>
 __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
@@ -351,8 +364,9 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
   const float kLog2e = 1.4426950408889634f;
   const int e0 = place.e0;
   uint32_t p[EPL];
-  const int bits = a.bias ? kScoreBits : 16;
-  uint32_t near = 0;  // values that differ by no more are not told apart
+  const bool rough = a.bias || sizeof(In) == 4;  // a key does not hold all of a value:
+  uint32_t near = 0;                             // values that differ by no more are not told apart
+  const int bits = rough ? kScoreBits : 16;
   if (a.bias) {
     const float kNaN = __int_as_float(0x7fffffff);
     float c[EPL], b[EPL];
@@ -429,26 +443,33 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
         const uint32_t h = __half_as_ushort(__float2half_rn(x[j] + 0.0f));
         v = ((h & 0x8000u) ? ~h : h | 0x8000u) & 0xffffu;
       } else {
-        v = key_of(x[j]) >> 16;
+        v = key_of(x[j]) >> (sizeof(In) == 4 ? kScoreBits : 16);
       }
-      p[j] = x[j] > neg_inf() ? (v << 16) | (0xffffu - (e0 + j)) : 0u;
+      constexpr int kBits = sizeof(In) == 4 ? kScoreBits : 16;
+      p[j] = x[j] > neg_inf() ? (v << kBits) | ((1u << kBits) - 1 - (e0 + j)) : 0u;
     }
   }
   sort_keys(p);
   const uint32_t mask = (1u << bits) - 1;
   auto exact = [&](int e) {
-    return exact_score(to_float(static_cast<const In*>(a.logits)[t * a.stride + e]),
-                       load_bias(a, e));
+    const float v = to_float(static_cast<const In*>(a.logits)[t * a.stride + e]);
+    return a.bias ? exact_score(v, load_bias(a, e)) : (double)v;
   };
   if (a.n_group > 1 && !a.bias && !a.group_max) {
     const int span = 1 << a.span_log2;
     uint32_t b1 = p[0], b2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] : 0u;
-    for (int o = 1; o < span; o <<= 1) {
-      const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
-      b2 = max(min(b1, q1), max(b2, q2));
-      b1 = max(b1, q1);
+    if constexpr (sizeof(In) == 4) {
+      uint32_t b3 = EPL > 2 ? p[EPL > 2 ? 2 : 0] : 0u;
+      for (int o = 1; o < span; o <<= 1) merge_best(b1, b2, b3, o);
+      if (__any_sync(kAll, b3 && (b2 >> bits) == (b3 >> bits))) return false;
+    } else {
+      for (int o = 1; o < span; o <<= 1) {
+        const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
+        b2 = max(min(b1, q1), max(b2, q2));
+        b1 = max(b1, q1);
+      }
     }
-    const int keep = keep_group(static_cast<const In*>(a.logits) + t * a.stride, b1, b2,
+    const int keep = keep_group(static_cast<const In*>(a.logits) + t * a.stride, b1, b2, mask,
                                 a.softmax, a.n_group, a.topk_group, a.span_log2, lane);
     if (keep < 0) return false;
     if (!keep) {
@@ -474,23 +495,15 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
     }
     for (int o = 1; o < span; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
     bool keep = rank < a.topk_group;
-    if (near) {
+    if (rough) {
       const uint32_t worst = __reduce_min_sync(kAll, keep ? mine : 0xffffffffu);
       const uint32_t best = __reduce_max_sync(kAll, keep ? 0u : mine);
       if (best > 0 && worst - best <= 2 * near) {
         // the groups' scores again, from their two best experts in 64 bits
-        if (a.softmax) return false;
+        if (a.softmax && a.bias) return false;
         uint32_t b1 = p[0], b2 = EPL > 1 ? p[EPL > 1 ? 1 : 0] : 0u;
         uint32_t b3 = EPL > 2 ? p[EPL > 2 ? 2 : 0] : 0u;
-        for (int o = 1; o < span; o <<= 1) {
-          const uint32_t q1 = __shfl_xor_sync(kAll, b1, o), q2 = __shfl_xor_sync(kAll, b2, o);
-          const uint32_t q3 = __shfl_xor_sync(kAll, b3, o);
-          // the three largest of two descending triples
-          const uint32_t low = min(b1, q1), mid = max(b2, q2);
-          b3 = max(max(min(low, mid), b3), max(q3, min(b2, q2)));
-          b2 = max(low, mid);
-          b1 = max(b1, q1);
-        }
+        for (int o = 1; o < span; o <<= 1) merge_best(b1, b2, b3, o);
         const uint32_t last = a.group_max ? b1 : b2, after = a.group_max ? b2 : b3;
         if (__any_sync(kAll, last && after && (last >> bits) - (after >> bits) <= near))
           return false;
@@ -515,7 +528,7 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
   // one round more than there are picks where a near runner-up matters; past the last usable
   // expert a round finds 0
   uint32_t last = 0, won = 0;
-  const int rounds = a.K + (near ? 1 : 0);
+  const int rounds = a.K + (rough ? 1 : 0);
 #pragma unroll 4
   for (int k = 0; k < rounds; ++k) {
     last = __reduce_max_sync(kAll, p[0]);
@@ -527,18 +540,19 @@ __device__ __forceinline__ bool select_by_key(const RouterArgs& a, int64_t t,
   }
   pick = won ? (int)(mask - (won & mask)) : -1;
   uint32_t gap = 0xffffffffu;  // the smallest of neighbours in the order
-  if (near) {
+  if (rough) {
     const uint32_t before = __shfl_up_sync(kAll, won, 1);
     if (lane > 0 && won) gap = before - won;
     if (rounds > 32 && lane == 31 && last) gap = min(gap, won - last);
     gap = __reduce_min_sync(kAll, gap);
   }
-  if (near && (gap >> bits) <= near) {
+  if (rough && (gap >> bits) <= near) {
     const int found = __popc(__ballot_sync(kAll, won != 0));
     // the picks and the runner-up in 64 bits, put in order by counting; the one behind them has to
     // be clear of them
     const uint32_t behind = __reduce_max_sync(kAll, p[0]);
-    if (a.softmax || rounds > 32 || (behind && (last >> bits) - (behind >> bits) <= near))
+    if ((a.softmax && a.bias) || rounds > 32 ||
+        (behind && (last >> bits) - (behind >> bits) <= near))
       return false;
     const double score = pick >= 0 ? exact(pick) : 0.0;
     int rank = 0;
@@ -753,7 +767,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32, router_blocks(EPL))
   load_logits<EPL, In>(a, t, place, x);
   int pick;
   bool sure;
-  if (a.by_key && (a.bias || sizeof(In) == 2))
+  if (a.by_key)
     sure = select_by_key<EPL, In>(a, t, x, place, lane, pick);
   else
     sure = select_experts<EPL, float>(a, x, place, lane, pick);

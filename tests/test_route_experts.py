@@ -173,6 +173,26 @@ def test_route_experts_groups_without_bias(fmoe, score, dtype, E, K, n, kg):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,K,n,kg,how", [(256, 8, 1, 1, "max"), (64, 32, 1, 1, "max"),
+                                          (160, 6, 8, 3, "top2"), (128, 8, 4, 2, "max"),
+                                          (384, 9, 2, 1, "top2"), (1024, 12, 32, 9, "max")])
+def test_route_experts_logits_that_share_their_upper_bits(fmoe, score, E, K, n, kg, how):
+    """fp32 logits without a bias: equal ones, ones a unit in the last place apart, and most of a
+    row at the type's lowest value."""
+    g = torch.Generator().manual_seed(E + K)
+    x = torch.randn(90, E, generator=g)
+    x[:30] = (x[:30] * 4).round() / 4
+    x[30:60] = (x[30:60] * 4).round() / 4
+    x[30:60] *= 1 + torch.randint(0, 3, (30, E), generator=g) * 2.0 ** -23
+    x[60:].masked_fill_(torch.rand(30, E, generator=g) < 0.95, torch.finfo(torch.float32).min)
+    idx, w = fmoe.route_experts(x.cuda(), K, score=score, n_group=n, topk_group=kg, group_score=how)
+    want_idx, want_w = ref.route(x, None, K, score, n, kg, how)
+    assert torch.equal(idx.cpu(), want_idx)
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_experts_infinite_logits(fmoe, score):
     x = torch.randn(4, 32, generator=torch.Generator().manual_seed(0))
     x[0, 7] = math.inf
