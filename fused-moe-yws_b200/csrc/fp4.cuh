@@ -133,7 +133,7 @@ __device__ __forceinline__ uint32_t nv_scale(uint32_t top, const NvDivisor& n, f
 template <int kFormat>
 __device__ __forceinline__ uint32_t encode16(float (&v)[16], uint32_t top, const NvDivisor& n,
                                              uint32_t& lo, uint32_t& hi) {
-  uint32_t byte;
+  uint32_t byte, flip = 0;
   float by;
   if constexpr (kFormat == FMOE_MXFP4) {
     byte = mx_scale(top, by);
@@ -143,8 +143,11 @@ __device__ __forceinline__ uint32_t encode16(float (&v)[16], uint32_t top, const
     byte = nv_scale(top, n, by);
     const float r = __frcp_rn(by);
     if (tame(by) && __int_as_float((int)top) * r < 0x1p20f) {
-      // two at a time: each half of a packed operation rounds like the single one
-      const float2 r2 = make_float2(r, r), d2 = make_float2(-by, -by);
+      // Two at a time: each half of a packed operation rounds like the single one. With -r for r
+      // all signs are turned, and a zero keeps its own (the residual step adds +0 to it, which
+      // would take it from -0).
+      const float2 r2 = make_float2(-r, -r), d2 = make_float2(by, by);
+      flip = 0x88888888u;
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const float2 x = make_float2(v[i], v[i + 1]);
@@ -161,8 +164,8 @@ __device__ __forceinline__ uint32_t encode16(float (&v)[16], uint32_t top, const
   }
   const float a[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
   const float b[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
-  lo = encode8(a);
-  hi = encode8(b);
+  lo = encode8(a) ^ flip;
+  hi = encode8(b) ^ flip;
   return byte;
 }
 

@@ -343,7 +343,8 @@ enum fmoe_dtype { FMOE_F32 = 0, FMOE_BF16 = 1, FMOE_F16 = 2 };
  *     two largest c (a group with fewer than two usable experts counts as -inf) or the largest;
  *   topk_idx = the top_k experts of the kept groups by c, largest first, -1 where none is left;
  *   topk_w = scale * s_k; with renormalize, scale * softmax over the picked experts, or for
- *     the sigmoid scale * s_k / (sum of the picked s + 1e-20); 0 beside an index of -1.
+ *     the sigmoid scale * s_k / (sum of the picked s + 1e-20), in fp32 (a sigmoid below 2^-126
+ *     counts as 0); 0 beside an index of -1.
  * Every choice goes to the larger value in exact arithmetic and to the lower index on a tie.
  * num_experts <= 1024, top_k and n_group <= 32. */
 enum fmoe_score { FMOE_SCORE_SOFTMAX = 0, FMOE_SCORE_SIGMOID = 1 };

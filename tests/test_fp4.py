@@ -51,6 +51,24 @@ def _check(q, x, fmt, g=None):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("g", [None, 2.0 ** -9, 2.0 ** 110])
+def test_zeros_keep_their_sign(fmoe, fmt, dtype, g):
+    """Zeros of both signs among other values, and alone; a global scale that takes the other way
+    to the quotients."""
+    if fmt == "mxfp4" and g is not None:
+        pytest.skip("mxfp4 has no global scale")
+    x = _values(40, 96, "normal", 1)
+    x = x * torch.randint(0, 2, x.shape, generator=torch.Generator().manual_seed(2))
+    x[3] = -0.0
+    x = x.to(dtype)
+    assert (torch.signbit(x) & (x == 0)).sum() > 500
+    gd = None if g is None else torch.tensor(g, device="cuda")
+    _check(fmoe.quantize_fp4(x.cuda(), fmt, global_scale=gd), x, fmt, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["normal", "ties", "range", "special"])
 @pytest.mark.parametrize("rows,cols", [(1, 32), (3, 64), (128, 256), (129, 288), (257, 1056)])
 def test_quantize_and_back(fmoe, fmt, dtype, kind, rows, cols):
