@@ -4,7 +4,7 @@
 //             start at a multiple of 128, the row tile of the products
 //   quantise  the pairs' hidden rows, gathered, to 4-bit blocks
 //   product 1 with W13, SwiGLU and quantisation to 4-bit blocks in its epilogue
-//   product 2 with W2, times the routing weight, to fp32 rows (bf16 in large batches)
+//   product 2 with W2, times the routing weight, to fp32 rows
 //   combine   a token's rows summed in the order of its picks
 //
 // Nothing returns to the host: the number of row tiles stays on the device, buffers are sized
@@ -146,8 +146,10 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_plan_rows_kernel(PlanArgs a)
   }
 }
 
-// out[t] = the sum of a token's rows in the order of its picks, from fp32 rows. A thread takes 8
-// columns (one sector of a row).
+// out[t] = the sum of a token's rows in the order of its picks, rounded once. The rows are fp32 at
+// every batch size: a token's result is the same whatever batch it is in. (Rows in bf16 would
+// halve them but add as much error again as the result's own rounding.) A thread takes 8 columns
+// (one sector of a row).
 __global__ void __launch_bounds__(128) fp4_combine_kernel(const int* token_row, const float* rows,
                                                           __nv_bfloat16* out, int H, int K) {
   __shared__ int s_row[32];
@@ -185,15 +187,6 @@ struct Layout {
 // product's epilogue. Otherwise they are a pass of their own over an fp32 product.
 bool fused(const fmoe_fp4_problem* p) { return p->intermediate_size % 128 == 0; }
 
-// The expert's rows in fp32, where they fit the cache between the product that writes them and
-// the sum that reads them: the result is rounded once. Larger batches round each row to bf16
-// too, which with k rows a token adds as much error again (2.4e-3 for 1.7e-3, of the plain
-// product in fp32), but halves 0.9 GB of rows each way for 4096 tokens with 8 local picks each (H
-// 7168, 32 experts): 986 us, 1158 with fp32 rows. At 16 and 256 tokens the two take as long.
-bool exact_rows(const fmoe_fp4_problem* p) {
-  return p->num_tokens * p->top_k * p->hidden_size * 4 <= (int64_t)64 << 20;
-}
-
 Layout layout_of(const fmoe_fp4_problem* p) {
   Layout L = {};
   const int64_t pairs = p->num_tokens * p->top_k;
@@ -218,7 +211,7 @@ Layout layout_of(const fmoe_fp4_problem* p) {
   L.hidden = take(fused(p) ? 0 : rows * 2 * p->intermediate_size * 4);
   L.cq = take(rows * (p->intermediate_size / 2));
   L.cs = take(tiles * fp4::tiles_across(p->intermediate_size, p->format) * fp4::kTileBytes);
-  L.ow = take(rows * p->hidden_size * (exact_rows(p) ? 4 : 2));
+  L.ow = take(rows * p->hidden_size * 4);
   L.total = off;
   return L;
 }
@@ -376,28 +369,13 @@ extern "C" int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensor
   g.ga = t->intermediate_scale;
   g.gb = t->w2_global;
   g.out = ws + L.ow;
-  g.dtype = exact_rows(p) ? FMOE_F32 : FMOE_BF16;
+  g.dtype = FMOE_F32;
   g.row_w = plan.row_w;
   if ((v = launch_fp4_gemm(g, stream)) != FMOE_OK) return v;
 
   const unsigned T = (unsigned)p->num_tokens;
-  if (exact_rows(p)) {
-    e = launch_pdl(fp4_combine_kernel, dim3(T, (unsigned)((H / 8 + 127) / 128)), dim3(128), 0,
-                   stream, (const int*)plan.token_row, reinterpret_cast<const float*>(ws + L.ow),
-                   static_cast<__nv_bfloat16*>(t->output), H, p->top_k);
-    return e == cudaSuccess ? FMOE_OK : cuda_failed(e);
-  }
-  CombineArgs c = {};
-  c.token_row = plan.token_row;
-  c.ow = reinterpret_cast<const __nv_bfloat16*>(ws + L.ow);
-  c.out = static_cast<__nv_bfloat16*>(t->output);
-  c.T = p->num_tokens;
-  c.H = H;
-  c.top_k = p->top_k;
-  e = p->num_tokens >= kCombineWideTokens
-          ? launch_pdl(combine_kernel<2>, dim3(T, (unsigned)((H / 8 + 255) / 256)), dim3(128), 0,
-                       stream, c)
-          : launch_pdl(combine_kernel<1>, dim3(T, (unsigned)((H / 8 + 127) / 128)), dim3(128), 0,
-                       stream, c);
+  e = launch_pdl(fp4_combine_kernel, dim3(T, (unsigned)((H / 8 + 127) / 128)), dim3(128), 0, stream,
+                 (const int*)plan.token_row, reinterpret_cast<const float*>(ws + L.ow),
+                 static_cast<__nv_bfloat16*>(t->output), H, p->top_k);
   return e == cudaSuccess ? FMOE_OK : cuda_failed(e);
 }

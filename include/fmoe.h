@@ -423,8 +423,7 @@ int fmoe_fp4_matmul(const fmoe_fp4_matrix* a, const fmoe_fp4_matrix* b, void* ou
  * FP8 weights) with hidden states quantised by the layer and both products in 4 bits.
  *   x     = the hidden rows, quantised with input_scale
  *   h     = (x W13[:I]^T) * silu(x W13[I:]^T), quantised with intermediate_scale
- *   out_t = sum_k w_k h W2^T over the picks of the local experts, in fp32 (the rows rounded to
- *           bf16 before they are summed where num_tokens * top_k * hidden_size exceeds 2^24)
+ *   out_t = sum_k w_k h W2^T over the picks of the local experts, in fp32, rounded once
  * Picks outside [local_expert_offset, local_expert_offset + num_local_experts) take no part;
  * an expert may be named twice. */
 typedef struct fmoe_fp4_problem {

@@ -283,6 +283,52 @@ def test_forward_fp4_rejects_arguments(fmoe):
         fmoe.forward_fp4(*args, out=torch.empty(5, 256, dtype=torch.bfloat16, device="cuda"))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("T,H,I,E,E_local,K,offset,route,dtype", [
+    (300, 7168, 128, 16, 16, 8, 0, "random", torch.bfloat16),
+    (1100, 2048, 128, 8, 8, 8, 0, "random", torch.bfloat16),
+    (1100, 2048, 160, 32, 8, 8, 8, "holes", torch.float16),
+    # a batch that just fits in 2^24 values of all picks' rows, and one that just does not
+    (512, 4096, 128, 16, 4, 8, 4, "random", torch.float32),
+    (513, 4096, 128, 16, 4, 8, 4, "random", torch.bfloat16),
+])
+def test_forward_fp4_large_batches(fmoe, fmt, T, H, I, E, E_local, K, offset, route, dtype):
+    """A token's result is that of the definition in large batches too, and bit for bit the one it
+    has in a small batch: every sum has an order of its own, whatever lies beside it."""
+    args, kw, state = _case(fmoe, T, H, I, E, E_local, K, fmt, dtype, T + H, offset, route)
+    out = fmoe.forward_fp4(*args, **kw)
+    assert torch.equal(out, fmoe.forward_fp4(*args, **kw))
+    x, idx, w = args[:3]
+    for part in (slice(0, 40), slice(T // 2, T // 2 + 1), slice(T - 24, T)):
+        some = fmoe.forward_fp4(x[part].clone(), idx[part].clone(), w[part].clone(), *args[3:],
+                                **kw)
+        assert torch.equal(some, out[part])
+        want, bound = _expected(*(v[part] for v in state[:3]), *state[3:])
+        assert ((some.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("T,H,K", [(20, 1024, 2), (300, 7168, 8), (2100, 4096, 2)])
+def test_forward_fp4_rounds_once(fmoe, fmt, T, H, K):
+    """Picks that nearly cancel. With the same expert picked with weights 1 and 2^-7 - 1, a row r
+    of fp32 gives r - r (1 - 2^-7): its roundings (the factor, two rows, the sum: 2^-24 |r| each)
+    are below 2^-14 of the result r 2^-7. One rounding to bf16 follows, as for the pick of weight
+    2^-7 alone: each is within half a step (2^-8) of its number, 2^-7 (1 + 2^-8) together."""
+    args, kw, _ = _case(fmoe, T, H, 128, 4, 4, 1, fmt, torch.bfloat16, 3)
+    x, one, _, w13, w2, _ = args
+    idx = torch.full((T, K), -1, dtype=torch.int32, device="cuda")
+    w = torch.zeros(T, K, device="cuda")
+    idx[:, 0] = idx[:, K - 1] = one[:, 0]
+    w[:, 0], w[:, K - 1] = 1.0, 2.0 ** -7 - 1.0
+    got = fmoe.forward_fp4(x, idx, w, w13, w2, **kw).double()
+    want = fmoe.forward_fp4(x, one, torch.full((T, 1), 2.0 ** -7, device="cuda"), w13, w2,
+                            **kw).double()
+    assert want.abs().max() > 0
+    assert ((got - want).abs() <= want.abs() * (2.0 ** -7 + 2.0 ** -13)).all()
+
+
 # ------------------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("field,value", [
     ("num_tokens", -1), ("num_tokens", 2 ** 20 + 1), ("hidden_size", 48), ("hidden_size", 0),
