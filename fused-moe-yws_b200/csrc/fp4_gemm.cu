@@ -230,6 +230,26 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The factor of a row's sums: two global scales and the row's weight. Their product may leave fp32
+// where the results do not (two scales of 3e-23 multiply to nothing). Then `digits` is the product
+// with an exponent that keeps a sum times it a normal number (sums of nvfp4 products lie in 2^-20 ..
+// 2^39, or are 0), and the result what is to be multiplied by after it, a power of two (beyond fp32
+// the results are 0 or infinite). Otherwise the result is the product, and `split` is false.
+__device__ __forceinline__ float factor_of(float ga, float gb, float w, bool& split,
+                                           float& digits) {
+  const float ab = ga * gb, all = ab * w;
+  split = false;
+  if (fminf(fabsf(ab), fabsf(all)) >= 0x1p-126f && fmaxf(fabsf(ab), fabsf(all)) < 0x1p127f)
+    return all;
+  const double d = (double)ga * (double)gb * (double)w;  // three floats' exponents fit
+  const int e = (int)(__double_as_longlong(d) >> 52 & 0x7ff) - 1023;
+  if (d == 0.0 || e > 1000) return (float)d;  // an infinity, NaN
+  const int low = max(-80, min(80, e));
+  split = true;
+  digits = (float)(d * __longlong_as_double((long long)(1023 + low - e) << 52));
+  return ldexpf(1.0f, min(e - low, 127));
+}
+
 // Stores columns n .. n + 31 of the warp's 32 rows; lane l holds row m0 + l of `rows` and its 32
 // values. Where rows are not whole 32-byte sectors the lanes exchange values (a 32 x 32
 // transposition in registers), so that a store writes neighbouring columns of one row: 24 tiles
@@ -612,8 +632,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row = q * 32 + lane;
       const int64_t m = (int64_t)t.m * 128 + row, m0 = m - lane;
       const int rows = t.rows - q * 32;  // of this warp's 32
-      float alpha = p.gb ? ga * p.gb[t.e] : ga;  // (loaded while the tile is multiplied)
-      if (p.row_w && row < t.rows) alpha *= p.row_w[m];
+      bool split;  // (loaded while the tile is multiplied)
+      float digits = 1.0f;
+      const float alpha = factor_of(ga, p.gb ? p.gb[t.e] : 1.0f,
+                                    p.row_w && row < t.rows ? p.row_w[m] : 1.0f, split, digits);
+      split = __any_sync(0xffffffffu, split);
       if (!mbar_wait(&tfull[n & 1], (n >> 1) & 1, abort_flag)) {
         ok = false;
         break;
@@ -621,6 +644,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1) * C::kAcc1 + ((uint32_t)(q * 32) << 16);
       const int n0 = t.n * BN;
+      if (__builtin_expect(split, false)) {
+        // the digits' part in place, before anyone reads: this warp's columns, or its gate and up
+        // columns. (A second multiplication wherever the sums are used, which no ordinary tile needs,
+        // took the expert layer of 16 tokens from 94 to 102 us by its code alone.)
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 8) {
+          const uint32_t at = acc + (kEpi == kSwiglu ? half * 64 + (c & 63) + (c & 64) * 2
+                                                     : half * (BN / 2) + c);
+          uint32_t v[8];
+          tmem_ld_32x32b<8>(at, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * digits);
+          tmem_st_32x32b_x8(at, v);
+        }
+        tmem_st_wait();
+      }
       if constexpr (kSplit > 1) {
         // ---- a tile that the cluster shares: rows 0..31, so only the warps of lanes 0..31
         static_assert(kEpi == kStore && !C::kOverlapped, "a cluster's tile");

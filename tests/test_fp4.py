@@ -249,6 +249,34 @@ def test_quantize_then_multiply(fmoe, fmt):
         assert torch.equal(held, call())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(7, 300, 2080), (32, 9000, 2048), (300, 300, 288),
+                                   (1000, 4000, 288), (33, 129, 96)])
+@pytest.mark.parametrize("ga,gb", [(2.6e-23, 2.6e-23), (3e-22, 4e-22), (1e-30, 1e-9),
+                                   (1e-45, 1e30), (1e-30, 1e33), (3e20, 4e18), (1e30, 1e35),
+                                   (1e-38, 1e-38)])
+def test_matmul_global_scales_of_any_size(fmoe, M, N, K, ga, gb):
+    """Global scales whose product leaves the range of normal fp32 numbers while the results are
+    in it, results that leave it, and zeros. The factor is applied in fp32 to the fp32 sum: at most
+    three more roundings (2^-24 each), and 2^-150 (fp32) or 2^-134 (bf16) where the result is below
+    the normal range, twice."""
+    ca, sa, a = _operand(M, K, "nvfp4", None, 11)
+    cb, sb, b = _operand(N, K, "nvfp4", None, 12)
+    ca[M // 2], a[M // 2] = 0, 0.0
+    qa, qb = _held(fmoe, ca, sa, "nvfp4", ga), _held(fmoe, cb, sb, "nvfp4", gb)
+    f = qa.global_scale.double().item() * qb.global_scale.double().item()
+    want, size = a @ b.t() * f, a.abs() @ b.abs().t() * f
+    for dtype, least in ((torch.float32, 2.0 ** -149), (torch.bfloat16, 2.0 ** -133)):
+        got = fmoe.matmul_fp4(qa, qb, dtype=dtype).cpu().double()
+        half, most = torch.finfo(dtype).eps / 2, torch.finfo(dtype).max
+        bound = want.abs() * (half + 3 * 2.0 ** -24) + size * K * 2.0 ** -23 * (1 + half) + least
+        assert (got[M // 2] == 0).all()
+        below, above = want.abs() + bound < most, want.abs() - bound > most * (1 + half)
+        off = (got - want).abs()
+        assert (off[below] <= bound[below]).all(), (off / bound)[below].max().item()
+        assert (got[above] == want[above].sign() * float("inf")).all()
+
+
 # ------------------------------------------------------------------------------ refusals
 def _matrix(**kw):
     from fmoe_b200.fp4 import FmoeFp4Matrix

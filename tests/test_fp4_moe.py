@@ -329,6 +329,40 @@ def test_forward_fp4_rounds_once(fmoe, fmt, T, H, K):
     assert ((got - want).abs() <= want.abs() * (2.0 ** -7 + 2.0 ** -13)).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("I", [128, 160])
+def test_forward_fp4_small_scales(fmoe, I):
+    """Global scales of the second product that multiply to less than fp32 holds, under routing
+    weights that bring the result back; and of the first that multiply to more, over zeros."""
+    T, H, E, K = 40, 256, 4, 2
+    g = torch.Generator().manual_seed(I)
+    x = torch.randn(T, H, generator=g) * 2.0 ** -33
+    x[5] = 0.0
+    idx = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(T)]).to(torch.int32)
+    w = (torch.rand(T, K, generator=g) + 0.1) * 2.0 ** 50
+    w13, w2 = _weights(E, 2 * I, H, "nvfp4", 1), _weights(E, H, I, "nvfp4", 2)
+    w2["g"], w2["values"] = w2["g"] * 2.0 ** -70, w2["values"] * 2.0 ** -70
+    gx = (x.abs().amax() / 2688).item()
+    v = ref.values(*ref.quantize(x, "nvfp4", gx), "nvfp4") * gx
+    h = torch.cat([v @ e[:I].t() * torch.nn.functional.silu(v @ e[I:].t()) for e in w13["values"]])
+    gc = torch.tensor(h.abs().amax().item() / 2688).item()
+    assert gc * w2["g"].max().item() < 2.0 ** -149  # nothing is left of the factor in fp32
+    call = lambda x, gx, gc, w13, w: fmoe.forward_fp4(  # noqa: E731
+        x.cuda(), idx.cuda(), w.cuda(), _held(fmoe, w13, "nvfp4"), _held(fmoe, w2, "nvfp4"),
+        input_scale=torch.tensor(gx, device="cuda"),
+        intermediate_scale=torch.tensor(gc, device="cuda"))
+    out = call(x, gx, gc, w13, w)
+    want, bound = _expected(x, idx, w, w13, w2, 0, "nvfp4", gx, gc)
+    off = (out.cpu().double() - want).abs()
+    assert (out[5] == 0).all() and 2.0 ** -90 < want.abs().max() < 2.0 ** -40
+    assert (off <= bound).all(), (off / bound).max().item()
+    assert off.pow(2).sum().sqrt() <= 0.02 * want.pow(2).sum().sqrt()  # as in test_forward_fp4
+    # 2^100 times 2^100 is an infinity; a row of zeros stays one
+    big = dict(w13, g=w13["g"] * 0 + 2.0 ** 100)
+    out = call(torch.zeros(T, H), 2.0 ** 100, 1.0, big, w)
+    assert (out == 0).all()
+
+
 # ------------------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("field,value", [
     ("num_tokens", -1), ("num_tokens", 2 ** 20 + 1), ("hidden_size", 48), ("hidden_size", 0),
