@@ -633,6 +633,8 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
   bool sure = true;
   if (by_group) {
     const int G = a.E / a.n_group;
+    // fewer than two usable experts: below all others, also where the one has a bias of +inf
+    auto two_best = [&](V m1, V m2) { return m2 > kNone ? m1 + m2 : kNone; };
     V mine = kNone;  // the score of the lane's group: lane g's, or lane / span's
     int own = lane, span = 1;
     // groups of whole lanes: the lanes of a group merge their two best
@@ -653,7 +655,7 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
         m1 = m1 < p1 ? p1 : m1;
         m2 = low > second ? low : second;
       }
-      mine = a.group_max ? m1 : m1 + m2;
+      mine = a.group_max ? m1 : two_best(m1, m2);
     } else {
       for (int g = 0; g < a.n_group; ++g) {
         V m1 = kNone, m2 = kNone;
@@ -673,7 +675,7 @@ __device__ __forceinline__ bool select_experts(const RouterArgs& a, const float 
           m1 = m1 < p1 ? p1 : m1;
           m2 = low > second ? low : second;
         }
-        if (lane == g) mine = a.group_max ? m1 : m1 + m2;
+        if (lane == g) mine = a.group_max ? m1 : two_best(m1, m2);
       }
     }
     int rank = 0;

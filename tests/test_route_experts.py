@@ -331,6 +331,37 @@ def test_route_experts_graph_and_streams(fmoe):
         assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,n,kg", [(32, 4, 1), (32, 4, 2), (30, 3, 1), (60, 6, 2), (256, 8, 4),
+                                    (24, 12, 5)])
+@pytest.mark.parametrize("how", ["top2", "max"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_experts_bias_of_infinity(fmoe, score, E, n, kg, how, dtype):
+    """A bias of +inf puts its expert first; a group with no other usable expert is below all
+    others by "top2" all the same. The others are out by their logits or by a bias of -inf."""
+    G = E // n
+    g = torch.Generator().manual_seed(E + n)
+    x = torch.randn(12, E, generator=g).to(dtype)
+    b = (torch.rand(E, generator=g) - 0.5) * 0.2
+    b[1] = math.inf
+    x[0, :G] = x[3, :G] = -math.inf
+    x[0, 1] = x[3, 1] = 0.5
+    x[4, :G] = -math.inf
+    x[5, 2 * G:] = -math.inf  # fewer usable experts than picks
+    x[5, 0] = math.nan
+    second = b.clone()
+    second[0:G] = -math.inf
+    second[1] = math.inf
+    second[E - 1] = math.inf
+    for bias in (b, second):
+        idx, w = fmoe.route_experts(x.cuda(), 2, score=score, bias=bias.cuda(), n_group=n,
+                                    topk_group=kg, group_score=how)
+        want_idx, want_w = ref.route(x, bias, 2, score, n, kg, how)
+        assert torch.equal(idx.cpu(), want_idx)
+        torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
+
+
 # ------------------------------------------------------------------------------ refusals
 def _router(fmoe, **kw):
     from fmoe_b200.router import FmoeRouter
