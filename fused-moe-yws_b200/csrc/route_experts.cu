@@ -304,7 +304,8 @@ __device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, 
   const int own = lane >> span_log2;
   const float x1 = b1 ? to_float(row[mask - (b1 & mask)]) : neg_inf();
   const float x2 = b2 ? to_float(row[mask - (b2 & mask)]) : neg_inf();
-  const float top = warp_max(x1);
+  // (either may be the larger one: fp32 keys leave out the last bits)
+  const float top = warp_max(fmaxf(x1, x2));
   if (softmax && !(fabsf(top) < 1e30f)) return -1;  // an infinity, or no expert at all
   auto score = [&](float x) {
     return softmax ? fast_exp2((x - top) * kLog2e)
@@ -319,7 +320,8 @@ __device__ __noinline__ int keep_group(const In* row, uint32_t b1, uint32_t b2, 
   }
   bool keep = rank < topk_group;
   const float worst = warp_min(keep ? mine : 4.0f), best = warp_max(keep ? -1.0f : mine);
-  if (best >= 0.0f && worst - best <= 16 * 0x1p-23f) {  // a score's error is 8 * 2^-24
+  // (scores are at most 1; a score's error is 8 * 2^-24)
+  if (best >= 0.0f && !(worst - best > 16 * 0x1p-23f)) {
     const double sum = !b2       ? -1.0
                        : softmax ? exact_share(x1, top) + exact_share(x2, top)
                                  : exact_score(x1, 0.0f) + exact_score(x2, 0.0f);

@@ -362,6 +362,34 @@ def test_route_experts_bias_of_infinity(fmoe, score, E, n, kg, how, dtype):
         torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,n,kg", [(64, 8, 1), (64, 8, 3), (256, 8, 4), (128, 2, 1), (60, 6, 2)])
+@pytest.mark.parametrize("base", [2.0 ** 22, 2.0 ** 17, 2.0 ** 14, -2.0 ** 20])
+def test_route_experts_large_logits_that_share_their_upper_bits(fmoe, score, E, n, kg, base):
+    """Groups whose two best logits agree in all but their last bits, the larger one at the higher
+    index, so far from zero that their difference is large."""
+    G = E // n
+    g = torch.Generator().manual_seed(E + n)
+    # the other experts: out of use, or far below and each with upper bits of its own
+    x = torch.full((64, E), -math.inf)
+    x[1::2] = -2.0 ** 30 * (1 + torch.arange(E) / 1024)
+    step = max(0.25, abs(base) * 2.0 ** -23)
+    low = base + torch.randint(0, 8, (64, n), generator=g) * step
+    up = torch.randint(0, 40, (64, n), generator=g) * step
+    up[:16] += 80.0
+    at = torch.randint(0, G // 2, (64, n), generator=g) + torch.arange(n) * G
+    x.scatter_(1, at, low)
+    x.scatter_(1, at + G // 2, low + up)
+    # two groups a step apart, the better one behind the other
+    x[0] = -math.inf
+    x[0, 0], x[0, G - 1], x[0, G], x[0, 2 * G - 1] = base, base + 100, base, base + 100 + 2 * step
+    idx, w = fmoe.route_experts(x.cuda(), 2, score=score, n_group=n, topk_group=kg)
+    want_idx, want_w = ref.route(x, None, 2, score, n, kg, "top2")
+    assert torch.equal(idx.cpu(), want_idx)
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
+
+
 # ------------------------------------------------------------------------------ refusals
 def _router(fmoe, **kw):
     from fmoe_b200.router import FmoeRouter
