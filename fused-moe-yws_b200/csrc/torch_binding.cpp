@@ -16,6 +16,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <cstdint>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -346,6 +348,8 @@ Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle 
   expect(w, "topk_w", {T, K}, at::kFloat, dev);
   const OptTensor gx = optional_of(input_scale, "input_scale");
   const OptTensor gc = optional_of(intermediate_scale, "intermediate_scale");
+  if (offset < 0 || offset > INT32_MAX)  // (of ids that are int32)
+    value_error("local_expert_offset must be in [0, 2^31), got " + std::to_string(offset));
   auto narrow = [](int64_t v) { return (int32_t)std::min<int64_t>(v, 1 << 30); };
   fmoe_fp4_problem p = {};
   p.num_tokens = T;
@@ -353,7 +357,7 @@ Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle 
   p.intermediate_size = narrow(I);
   p.num_local_experts = narrow(E);
   p.top_k = narrow(K);
-  p.local_expert_offset = narrow(offset);
+  p.local_expert_offset = (int32_t)offset;
   p.format = f13;
   p.dtype = dtype;
   fmoe_fp4_tensors t = {};

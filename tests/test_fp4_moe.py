@@ -404,3 +404,26 @@ def test_fp4_forward_rejects_pointers(fmoe):
     assert call(t) == fmoe.FMOE_ERR_VALUE
     p.num_tokens = 0
     assert call(FmoeFp4Tensors()) == fmoe.FMOE_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [-1, -2 ** 31, -2 ** 32, -2 ** 40 - 1, 2 ** 31,
+                                    2 ** 32])
+def test_forward_fp4_rejects_offsets(fmoe, offset):
+    """Offsets that no expert id reaches, also where their low 32 bits are a valid one."""
+    args, kw, _ = _case(fmoe, 6, 256, 128, 16, 16, 4, "nvfp4", torch.bfloat16, 1)
+    with pytest.raises(ValueError, match="local_expert_offset"):
+        fmoe.forward_fp4(*args[:5], offset, **kw)
+
+
+@pytest.mark.gpu
+def test_forward_fp4_takes_large_offsets(fmoe):
+    """Ids up to the largest int32, told apart from those beside the slice."""
+    args, kw, _ = _case(fmoe, 9, 256, 128, 16, 16, 4, "nvfp4", torch.bfloat16, 1)
+    x, idx, w, w13, w2, _ = args
+    want = fmoe.forward_fp4(*args, **kw)
+    for offset in (2 ** 30 + 5, 2 ** 31 - 16):
+        far = idx + offset
+        assert torch.equal(fmoe.forward_fp4(x, far, w, w13, w2, offset, **kw), want)
+        assert (fmoe.forward_fp4(x, idx, w, w13, w2, offset, **kw) == 0).all()
+        assert (fmoe.forward_fp4(x, far, w, w13, w2, 2 ** 30 - 16, **kw) == 0).all()
