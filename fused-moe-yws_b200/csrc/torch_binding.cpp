@@ -379,9 +379,14 @@ Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle 
     if (workspace.device() != dev || !workspace.is_contiguous())
       value_error("workspace must be contiguous on " + dev.str());
   }
+  // the C call asks for 16-byte alignment; some tokens' part of a routing may have 4
+  auto aligned = [](const Tensor& v) {
+    return reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 ? v.clone() : v;
+  };
+  const Tensor idx16 = aligned(idx), w16 = aligned(w);
   t.hidden_states = x.data_ptr();
-  t.topk_idx = idx.data_ptr<int32_t>();
-  t.topk_w = w.data_ptr<float>();
+  t.topk_idx = idx16.data_ptr<int32_t>();
+  t.topk_w = w16.data_ptr<float>();
   t.w13 = w13.m.codes;
   t.w13_scales = w13.m.scales;
   t.w13_global = w13.m.global_scale;

@@ -363,6 +363,28 @@ def test_forward_fp4_small_scales(fmoe, I):
     assert (out == 0).all()
 
 
+@pytest.mark.gpu
+def test_forward_fp4_takes_slices_of_a_routing(fmoe):
+    """Picks and weights of some of a batch's tokens, at addresses of no more than 4 bytes'
+    alignment, also where a captured graph replays on new ones."""
+    args, kw, _ = _case(fmoe, 30, 256, 128, 16, 16, 3, "nvfp4", torch.bfloat16, 1)
+    x, idx, w = args[:3]
+    whole = fmoe.forward_fp4(*args, **kw)
+    for first, last in ((1, 30), (2, 11), (29, 30)):
+        part = slice(first, last)
+        assert idx[part].data_ptr() % 16
+        assert torch.equal(fmoe.forward_fp4(x[part], idx[part], w[part], *args[3:], **kw),
+                           whole[part])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = fmoe.forward_fp4(x[1:], idx[1:], w[1:], *args[3:], **kw)
+    for _ in range(2):
+        idx.copy_(idx.roll(3, 0))
+        w.copy_(w.flip(0))
+        graph.replay()
+        assert torch.equal(held, fmoe.forward_fp4(*args, **kw)[1:])
+
+
 # ------------------------------------------------------------------------------ refusals
 @pytest.mark.parametrize("field,value", [
     ("num_tokens", -1), ("num_tokens", 2 ** 20 + 1), ("hidden_size", 48), ("hidden_size", 0),
