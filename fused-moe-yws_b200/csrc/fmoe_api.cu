@@ -163,8 +163,8 @@ int num_sms_current() {
 // One host-mapped pinned pair {error bits, report count} per device. The combine kernel of
 // every call adds its call's device error word to it (report_device_error), so a timeout
 // inside a GEMM reaches the host without a synchronisation: fmoe_poll_device_error() reads
-// the pair. It is allocated on a device's first call that is not being captured into a
-// graph (a capturing stream cannot allocate); calls captured before that report nothing.
+// the pair. It is allocated by a device's first poll, or its first call that is not being
+// captured into a graph; calls captured before that report nothing.
 struct ErrorSink {
   unsigned* host = nullptr;  // [0] bits, [1] count
   unsigned* dev = nullptr;
@@ -183,9 +183,14 @@ unsigned* error_sink_for(int dev, cudaStream_t stream) {
     if (cudaStreamIsCapturing(stream, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
       return nullptr;
   }
+  // a poll may come while a stream is captured, which an allocation in the default mode would break
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
   void* h = nullptr;
-  if (cudaHostAlloc(&h, 2 * sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable) !=
-      cudaSuccess) {
+  const cudaError_t made =
+      cudaHostAlloc(&h, 2 * sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable);
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+  if (made != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }

@@ -183,8 +183,9 @@ int fmoe_read_device_error(const fmoe_problem* p, void* workspace, void* stream,
  * calls still running. The reference raises RuntimeError for every CUDA error
  * (kernel.cu:53-62) after a full stream synchronisation (kernel.cu:1834); the TVM-FFI
  * binding and the Python mirror poll at the start of every call and raise then. The word
- * is allocated (8 bytes of pinned host memory) by a device's first call or poll that is not
- * inside a stream capture; calls captured into a graph before that report nothing. */
+ * is allocated (8 bytes of pinned host memory) by a device's first poll, or its first call
+ * that is not inside a stream capture; calls captured into a graph before that report nothing.
+ * A poll may come while a stream is being captured. */
 int fmoe_poll_device_error(int32_t* device_error);
 
 /* Test hook for the error path above (no fault, no hang): the next fmoe_forward() or

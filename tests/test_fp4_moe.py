@@ -9,6 +9,10 @@ rounded as in 64 bits. The second product, the weight and the sum over the picks
 magnitudes, each row rounded to bf16 (2^-9... eps / 2 = 2^-8 of the magnitudes), the sum again.
 """
 import ctypes
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -383,6 +387,37 @@ def test_forward_fp4_takes_slices_of_a_routing(fmoe):
         w.copy_(w.flip(0))
         graph.replay()
         assert torch.equal(held, fmoe.forward_fp4(*args, **kw)[1:])
+
+
+@pytest.mark.gpu
+def test_fp4_first_call_of_a_process_can_be_captured(fmoe):
+    """Nothing that a call makes for later calls (the device's error word) may break a capture.
+    In a process of its own, where no call came before."""
+    program = """
+import torch
+import fmoe_b200 as f
+x = torch.randn(40, 256, device="cuda")
+w13, w2 = torch.randn(4, 256, 256, device="cuda") / 16, torch.randn(4, 256, 128, device="cuda") / 11
+idx = torch.arange(80, device="cuda", dtype=torch.int32).view(40, 2) % 4
+w = torch.full((40, 2), 0.5, device="cuda")
+f.load_library()
+torch.cuda.synchronize()
+def call():
+    q = f.quantize_fp4(x, "nvfp4")
+    return f.matmul_fp4(q, q), f.forward_fp4(x, idx, w, f.quantize_fp4(w13, "nvfp4"),
+                                             f.quantize_fp4(w2, "nvfp4"))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = call()
+graph.replay()
+for a, b in zip(held, call()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+    root = Path(fmoe.__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PYTHONPATH=str(root)))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------------------ refusals
