@@ -292,22 +292,6 @@ Tensor dequantize_fp4(py::handle codes, py::handle scales, py::handle global, in
   return out;
 }
 
-Tensor matmul_fp4(py::handle a_codes, py::handle a_scales, py::handle a_global, int a_format,
-                  py::handle b_codes, py::handle b_scales, py::handle b_global, int b_format,
-                  py::handle dtype_h, py::handle out_h) {
-  const Matrix a = matrix_of(a_codes, a_scales, a_global, a_format, 2, "a");
-  const Matrix b = matrix_of(b_codes, b_scales, b_global, b_format, 2, "b");
-  const c10::Device dev = a.codes.device();
-  if (b.codes.device() != dev) value_error("a and b must be on the same device");
-  const at::ScalarType dtype = scalar_type(dtype_h);
-  c10::cuda::CUDAGuard guard(dev);
-  Tensor out = out_of(out_h, {a.m.rows, b.m.rows}, dtype, dev);
-  const int rc =
-      fmoe_fp4_matmul(&a.m, &b.m, out.data_ptr(), dtype_code(dtype, "output"), stream_of(dev));
-  if (rc != FMOE_OK) raise("matmul_fp4", rc);
-  return out;
-}
-
 void raise_device_error(c10::Device dev, const char* when) {
   int32_t bits = 0;
   const int rc = fmoe_poll_device_error(&bits);
@@ -321,6 +305,33 @@ void raise_device_error(c10::Device dev, const char* when) {
                                " (a bounded wait expired); that call's output is invalid")
                                   .c_str());
   throw py::error_already_set();
+}
+
+// Waits for the current stream, where the caller wants to hear of this call's own errors.
+void check_call(c10::Device dev) {
+  {
+    py::gil_scoped_release release;
+    c10::cuda::getCurrentCUDAStream(dev.index()).synchronize();
+  }
+  raise_device_error(dev, "this call");
+}
+
+Tensor matmul_fp4(py::handle a_codes, py::handle a_scales, py::handle a_global, int a_format,
+                  py::handle b_codes, py::handle b_scales, py::handle b_global, int b_format,
+                  py::handle dtype_h, py::handle out_h, bool check) {
+  const Matrix a = matrix_of(a_codes, a_scales, a_global, a_format, 2, "a");
+  const Matrix b = matrix_of(b_codes, b_scales, b_global, b_format, 2, "b");
+  const c10::Device dev = a.codes.device();
+  if (b.codes.device() != dev) value_error("a and b must be on the same device");
+  const at::ScalarType dtype = scalar_type(dtype_h);
+  c10::cuda::CUDAGuard guard(dev);
+  raise_device_error(dev, "an earlier call on this device");
+  Tensor out = out_of(out_h, {a.m.rows, b.m.rows}, dtype, dev);
+  const int rc =
+      fmoe_fp4_matmul(&a.m, &b.m, out.data_ptr(), dtype_code(dtype, "output"), stream_of(dev));
+  if (rc != FMOE_OK) raise("matmul_fp4", rc);
+  if (check) check_call(dev);
+  return out;
 }
 
 Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle c13, py::handle s13,
@@ -396,11 +407,7 @@ Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle 
   t.output = out.data_ptr();
   rc = fmoe_fp4_forward(&p, &t, workspace.data_ptr(), workspace.nbytes(), stream_of(dev));
   if (rc != FMOE_OK) raise("forward_fp4", rc);
-  if (check) {
-    py::gil_scoped_release release;
-    c10::cuda::getCurrentCUDAStream(dev.index()).synchronize();
-  }
-  if (check) raise_device_error(dev, "this call");
+  if (check) check_call(dev);
   return out;
 }
 

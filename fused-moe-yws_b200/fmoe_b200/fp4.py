@@ -111,14 +111,15 @@ def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
 
 
 def matmul_fp4(a: Fp4Tensor, b: Fp4Tensor, *, dtype: torch.dtype = torch.bfloat16,
-               out: torch.Tensor | None = None) -> torch.Tensor:
-    """``a`` [M, K] times the transpose of ``b`` [N, K], summed in fp32, in ``dtype``."""
+               out: torch.Tensor | None = None, check: bool = False) -> torch.Tensor:
+    """``a`` [M, K] times the transpose of ``b`` [N, K], summed in fp32, in ``dtype``. ``check`` as
+    in ``kernel``; a device error of an earlier call raises ``DeviceError``."""
     for name, m in (("a", a), ("b", b)):
         if not isinstance(m, Fp4Tensor):
             raise ValueError(f"{name} must be an Fp4Tensor")
     return (router._module or binding()).matmul_fp4(
         a.codes, a.scales, a.global_scale, code(FORMATS, a.format, "format"), b.codes, b.scales,
-        b.global_scale, code(FORMATS, b.format, "format"), dtype, out)
+        b.global_scale, code(FORMATS, b.format, "format"), dtype, out, check)
 
 
 def fp4_workspace_bytes(prob: FmoeFp4Problem) -> int:

@@ -277,6 +277,28 @@ def test_matmul_global_scales_of_any_size(fmoe, M, N, K, ga, gb):
         assert (got[above] == want[above].sign() * float("inf")).all()
 
 
+@pytest.mark.gpu
+def test_matmul_fp4_reports_device_errors(fmoe):
+    """An error that an earlier call left (planted on the host) is raised by a product too, once;
+    check=True waits for the call itself."""
+    from fmoe_b200 import workloads as W
+
+    geo = W.TINY
+    inp = W.make_inputs(geo, 16, seed=3)
+    gpu = {k: v.cuda() for k, v in inp.items() if isinstance(v, torch.Tensor)}
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(0)).cuda()
+    q = fmoe.quantize_fp4(x, "nvfp4")
+    want = fmoe.matmul_fp4(q, q)
+    assert fmoe.poll_device_error() == 0
+    fmoe.inject_device_error(1 << 1)
+    fmoe.kernel(*W.operator_args(gpu), 0, 2.5)
+    torch.cuda.synchronize()
+    with pytest.raises(fmoe.DeviceError, match="device error 0x2"):
+        fmoe.matmul_fp4(q, q)
+    assert torch.equal(fmoe.matmul_fp4(q, q, check=True), want)
+    assert fmoe.poll_device_error() == 0
+
+
 # ------------------------------------------------------------------------------ refusals
 def _matrix(**kw):
     from fmoe_b200.fp4 import FmoeFp4Matrix
