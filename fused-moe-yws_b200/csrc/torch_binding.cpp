@@ -10,6 +10,8 @@
 // word.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -86,6 +88,12 @@ void* stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.in
 // (at::empty without its dispatch, 0.4 us a tensor)
 Tensor empty(c10::IntArrayRef shape, at::ScalarType dtype, c10::Device dev) {
   return at::detail::empty_cuda(shape, dtype, dev, std::nullopt);
+}
+
+// A dual tensor's tangent would be lost: no operator here has a forward-mode derivative.
+void refuse_tangent(const Tensor& t, const std::string& name) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    value_error(name + " carries a forward-mode tangent, which this operator does not pass on");
 }
 
 // ------------------------------------------------------------------------------- router
@@ -334,6 +342,14 @@ Tensor matmul_fp4(py::handle a_codes, py::handle a_scales, py::handle a_global, 
   return out;
 }
 
+// The layer has no derivative: a graph that ends here without a word would train nothing.
+void refuse_gradient(const Tensor& t, const std::string& name) {
+  refuse_tangent(t, name);
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    value_error(name + " requires a gradient, and forward_fp4 has no gradient: detach it, or call "
+                       "under torch.no_grad()");
+}
+
 Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle c13, py::handle s13,
                    py::handle g13, int f13, py::handle c2, py::handle s2, py::handle g2, int f2,
                    int64_t offset, py::handle input_scale, py::handle intermediate_scale,
@@ -345,6 +361,8 @@ Tensor forward_fp4(py::handle x_h, py::handle idx_h, py::handle w_h, py::handle 
     value_error("topk_idx must be 2D");
   const Tensor x = THPVariable_Unpack(x_h.ptr()), idx = THPVariable_Unpack(idx_h.ptr());
   const Tensor w = tensor_of(w_h, "topk_w");
+  refuse_gradient(x, "hidden_states");
+  refuse_gradient(w, "topk_w");
   const int dtype = dtype_code(x.scalar_type(), "hidden_states");
   const Matrix w13 = matrix_of(c13, s13, g13, f13, 3, "w13"), w2 = matrix_of(c2, s2, g2, f2, 3, "w2");
   const c10::Device dev = w13.codes.device();

@@ -144,6 +144,8 @@ def forward_fp4(hidden_states: torch.Tensor, topk_idx: torch.Tensor, topk_w: tor
     rows, then up rows; the SiLU is on the up half, as in ``kernel``) and ``w2`` [E_local, H, I]
     hold experts [offset, offset + E_local); picks outside take no part. ``input_scale`` and
     ``intermediate_scale`` (nvfp4, fp32 [1] on the device) are the activations' global scales.
+    There is no backward pass: ``hidden_states`` or ``topk_w`` that require a gradient are refused
+    outside ``torch.no_grad()``.
     ``workspace`` is the caller's scratch (``fp4_workspace_bytes``; one call at a time), ``check``
     as in ``kernel``; a device error of an earlier call raises ``DeviceError``."""
     for name, m in (("w13", w13), ("w2", w2)):

@@ -484,3 +484,26 @@ def test_forward_fp4_takes_large_offsets(fmoe):
         assert torch.equal(fmoe.forward_fp4(x, far, w, w13, w2, offset, **kw), want)
         assert (fmoe.forward_fp4(x, idx, w, w13, w2, offset, **kw) == 0).all()
         assert (fmoe.forward_fp4(x, far, w, w13, w2, 2 ** 30 - 16, **kw) == 0).all()
+
+
+@pytest.mark.gpu
+def test_forward_fp4_refuses_to_drop_a_gradient(fmoe):
+    """The layer has no backward pass: what would ask it for one is refused, not cut off."""
+    args, kw, _ = _case(fmoe, 6, 256, 128, 16, 16, 4, "nvfp4", torch.bfloat16, 1)
+    x, idx, w, w13, w2, _ = args
+    want = fmoe.forward_fp4(*args, **kw)
+    logits = torch.randn(6, 16, device="cuda", requires_grad=True)
+    idx2, w2_ = fmoe.route_experts(logits, 4)
+    for xx, ii, ww in ((x.clone().requires_grad_(True), idx, w), (x, idx2, w2_)):
+        with pytest.raises(ValueError, match="no gradient"):
+            fmoe.forward_fp4(xx, ii, ww, w13, w2, **kw)
+    # without a graph to lose, the same tensors are taken
+    with torch.no_grad():
+        assert torch.equal(fmoe.forward_fp4(x.clone().requires_grad_(True), idx, w, w13, w2, **kw),
+                           want)
+    assert fmoe.forward_fp4(x, idx2, w2_.detach(), w13, w2, **kw).shape == x.shape
+    with torch.autograd.forward_ad.dual_level():
+        for name, (xx, ww) in {"hidden_states": (torch.autograd.forward_ad.make_dual(x, x), w),
+                               "topk_w": (x, torch.autograd.forward_ad.make_dual(w, w))}.items():
+            with pytest.raises(ValueError, match=name + ".*tangent"):
+                fmoe.forward_fp4(xx, idx, ww, w13, w2, **kw)
