@@ -101,6 +101,7 @@ Tensor logits_of(py::handle h) {
   if (!THPVariable_Check(h.ptr()) || THPVariable_Unpack(h.ptr()).dim() != 2)
     value_error("logits must be 2D");
   Tensor x = THPVariable_Unpack(h.ptr());
+  refuse_tangent(x, "logits");
   if (!x.is_cuda()) value_error("logits must be a CUDA tensor");
   // rows may be padded; anything else (transposed, broadcast) is laid out first
   const int64_t T = x.size(0), E = x.size(1);
@@ -166,6 +167,7 @@ Tensor route_experts_backward(py::handle grad_h, py::handle logits, py::handle i
       router_of(x, K, score, 1, 1, FMOE_GROUP_TOP2, renormalize, scale);
   expect(idx, "topk_idx", {T, K}, at::kInt, dev);
   const Tensor grad = tensor_of(grad_h, "grad_w").contiguous();  // it may arrive broadcast
+  refuse_tangent(grad, "grad_w");
   expect(grad, "grad_w", {T, K}, at::kFloat, dev);
   c10::cuda::CUDAGuard guard(dev);
   Tensor out = empty({T, x.size(1)}, x.scalar_type(), dev);

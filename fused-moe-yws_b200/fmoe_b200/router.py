@@ -101,9 +101,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     experts gets -1 with weight 0 in the places left, ties go to the lower index and the order is
     that of exact arithmetic. ``group_score`` is "top2" (sum of a group's two best) or "max".
     With ``renormalize`` the picked weights sum to ``scale``. Differentiable in the logits, the
-    picks held fixed; the bias gets no gradient. The results go to ``forward_fp4`` or
-    ``forward_routed``, which have no backward pass; the gradient is for a training program's own
-    expert layer."""
+    picks held fixed, in reverse mode alone (a forward-mode tangent is refused); the bias gets no
+    gradient. The results go to ``forward_fp4`` or ``forward_routed``, which have no backward pass;
+    the gradient is for a training program's own expert layer."""
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return _RouteExperts.apply(logits, bias, top_k, score, n_group, topk_group, group_score,
                                    renormalize, scale)

@@ -465,3 +465,31 @@ def test_route_experts_rejects_arguments(fmoe):
         fmoe.route_experts_backward(torch.zeros(4, 3, device="cuda"), x, idx)
     with pytest.raises(TypeError, match="grad_w"):
         fmoe.route_experts_backward(torch.zeros(4, 2, device="cuda").half(), x, idx)
+
+
+def test_route_experts_refuses_forward_mode(fmoe):
+    """A tangent would be lost without a word: there is no forward-mode derivative."""
+    x = torch.randn(4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError, match="logits.*tangent"):
+            fmoe.route_experts(torch.autograd.forward_ad.make_dual(x, x), 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        fmoe.route_experts(x, 2)
+
+
+@pytest.mark.gpu
+def test_route_experts_refuses_forward_mode_on_the_device(fmoe):
+    """Also with a reverse-mode leaf (torch refuses that one itself); the same tensors without
+    their tangents are taken."""
+    x = torch.randn(4, 8, device="cuda")
+    idx, w = fmoe.route_experts(x, 2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        leaf = torch.autograd.forward_ad.make_dual(x.clone().requires_grad_(True), x)
+        for logits in (dual, leaf):
+            with pytest.raises((ValueError, RuntimeError)):
+                fmoe.route_experts(logits, 2)
+        with pytest.raises(ValueError, match="grad_w.*tangent"):
+            fmoe.route_experts_backward(torch.autograd.forward_ad.make_dual(w, w), x, idx)
+        primal = torch.autograd.forward_ad.unpack_dual(dual).primal
+        assert torch.equal(fmoe.route_experts(primal, 2)[0], idx)
