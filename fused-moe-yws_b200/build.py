@@ -7,7 +7,8 @@ Produces, inside ``fused-moe-yws_b200/lib``:
   relies on IEEE single-precision rounding).
 * ``libfmoe_tvm_ffi.so`` -- the TVM-FFI ``kernel`` export with the reference signature,
   built only when the ``tvm_ffi`` headers are importable.
-* ``fmoe_torch.so`` -- the compiled Python entry points of the router and the 4-bit operators.
+* ``fmoe_torch.so`` -- the compiled Python entry points of the router and the 4-bit operators,
+  built only where torch with its C++ headers and CUDA libraries is installed.
 
 Run ``python fused-moe-yws_b200/build.py`` or call ``build()``.
 """
@@ -94,15 +95,27 @@ def build_tvm_ffi(verbose: bool = False):
     return so
 
 
-def build_torch(verbose: bool = False) -> Path:
-    """The compiled Python entry points of the router and the 4-bit operators (fmoe_torch.so)."""
+def build_torch(verbose: bool = False):
+    """The compiled Python entry points of the router and the 4-bit operators (fmoe_torch.so), or
+    None where there is no torch to build against: the C library does without."""
     import sysconfig
 
-    import torch
-
-    root = Path(torch.__file__).resolve().parent
-    src = CSRC / "torch_binding.cpp"
     so = LIB / "fmoe_torch.so"
+    try:
+        import torch
+    except ImportError:
+        print(f"[fmoe build] {so.name} left out: torch cannot be imported")
+        return None
+    root = Path(torch.__file__).resolve().parent
+    for need in ("include/torch/csrc/utils/pybind.h", "lib/libc10_cuda.so"):
+        if not (root / need).exists():
+            print(f"[fmoe build] {so.name} left out: torch has no {need}")
+            return None
+    src = CSRC / "torch_binding.cpp"
+    # the binding fits the torch it was compiled against alone
+    stamp, version = LIB / "fmoe_torch.version", torch.__version__
+    if not stamp.exists() or stamp.read_text() != version:
+        so.unlink(missing_ok=True)
     if _stale(so, [src, INCLUDE / "fmoe.h"]):
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", str(src), "-o",
                str(so), f"-I{INCLUDE}", f"-I{CUDA_HOME / 'include'}", f"-I{root / 'include'}",
@@ -112,6 +125,7 @@ def build_torch(verbose: bool = False) -> Path:
                f"-L{LIB}", "-lfmoe", f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
                "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{root / 'lib'}"]
         subprocess.check_call(cmd)
+        stamp.write_text(version)
         if verbose:
             print(f"[fmoe build] linked {so}")
     return so

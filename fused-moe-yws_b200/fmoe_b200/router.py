@@ -40,6 +40,10 @@ def binding():
         if not path.exists():
             raise RuntimeError(f"torch binding not built: {path} (run `python "
                                f"fused-moe-yws_b200/build.py`)")
+        built = path.with_suffix(".version")  # compiled code of another torch may crash this one
+        if built.exists() and built.read_text() != torch.__version__:
+            raise RuntimeError(f"torch binding built for torch {built.read_text()}, this is "
+                               f"{torch.__version__} (run `python fused-moe-yws_b200/build.py`)")
         loader = importlib.machinery.ExtensionFileLoader("fmoe_torch", str(path))
         spec = importlib.util.spec_from_file_location("fmoe_torch", path, loader=loader)
         module = importlib.util.module_from_spec(spec)
