@@ -7,10 +7,10 @@
 //   w_k = scale * s_k, or renormalised: softmax over the picked experts; for the sigmoid
 //         scale * s_k / (sum_k s_k + 1e-20)
 //
-// The order is decided as exact arithmetic decides it: two scores that differ by less than
-// single precision resolves still have an order, and a different pick changes the token's
-// output. Scores are computed in single precision with a bound on their error; what lies within
-// it of a neighbour that matters is decided in 64 bits.
+// The order is that of 64-bit arithmetic: two scores that differ by less than single precision
+// resolves still have an order, and a different pick changes the token's output. Scores are
+// computed in single precision with a bound on their error; what lies within it of a neighbour that
+// matters is decided in 64 bits (where sigmoids above a logit of 37 are 1, and tie).
 //
 // One warp routes one token, a lane holds up to EPL consecutive experts; where the number of
 // groups is a power of two, 32 / n_group lanes hold a group's (Place), so that groups of any size

@@ -103,7 +103,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     the scores for the choice only. The rule is that of fmoe_route_experts (include/fmoe.h): an
     expert with a logit of -inf or NaN is never picked, a token with fewer than ``top_k`` usable
     experts gets -1 with weight 0 in the places left, ties go to the lower index and the order is
-    that of exact arithmetic. ``group_score`` is "top2" (sum of a group's two best) or "max".
+    that of the logits, with a bias that of the biased scores in 64 bits. ``group_score`` is "top2" (sum of a group's two best) or "max".
     With ``renormalize`` the picked weights sum to ``scale``. Differentiable in the logits, the
     picks held fixed, in reverse mode alone (a forward-mode tangent is refused); the bias gets no
     gradient. The results go to ``forward_fp4`` or ``forward_routed``, which have no backward pass;

@@ -346,7 +346,10 @@ enum fmoe_dtype { FMOE_F32 = 0, FMOE_BF16 = 1, FMOE_F16 = 2 };
  *   topk_w = scale * s_k; with renormalize, scale * softmax over the picked experts, or for
  *     the sigmoid scale * s_k / (sum of the picked s + 1e-20), in fp32 (a sigmoid below 2^-126
  *     counts as 0); 0 beside an index of -1.
- * Every choice goes to the larger value in exact arithmetic and to the lower index on a tie.
+ * Every choice goes to the larger value and to the lower index on a tie. c and its sums are
+ * compared as 64-bit arithmetic gives them: what differs by less than about 2^-52 of c ties (a
+ * sigmoid of a logit above 37 is 1, of one below -709 it is 0). Without a bias the logits are
+ * compared as they are, and only the groups' sums are of that kind.
  * num_experts <= 1024, top_k and n_group <= 32. */
 enum fmoe_score { FMOE_SCORE_SOFTMAX = 0, FMOE_SCORE_SIGMOID = 1 };
 enum fmoe_group_score { FMOE_GROUP_TOP2 = 0, FMOE_GROUP_MAX = 1 };

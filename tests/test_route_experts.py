@@ -390,6 +390,26 @@ def test_route_experts_large_logits_that_share_their_upper_bits(fmoe, score, E, 
     torch.testing.assert_close(w.cpu().double(), want_w, rtol=REL, atol=2.0 ** -100)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,kg", [(1, 1), (4, 4), (3, 3)])
+def test_route_experts_scores_that_64_bits_do_not_tell_apart(fmoe, n, kg):
+    """Biased scores are compared as 64 bits hold them: sigmoids of 40 and 41 are both 1, and a
+    share of 2^-60 is nothing beside a bias of 1. Without a bias the logits themselves decide."""
+    E = 48
+    x = torch.full((2, E), -3.0)
+    x[0, 3], x[0, 40] = 40.0, 41.0
+    x[1, 5], x[1, 44] = -44.0, -43.0
+    b = torch.zeros(E)
+    b[5] = b[44] = 1.0
+    for bias, first in ((None, [[40, 3], None]), (b * 0, [[3, 40], None]), (b, [None, [5, 44]])):
+        idx, _ = fmoe.route_experts(x.cuda(), 2, score="sigmoid", n_group=n, topk_group=kg,
+                                    bias=None if bias is None else bias.cuda())
+        want, _ = ref.route(x, bias, 2, "sigmoid", n, kg)
+        assert torch.equal(idx.cpu(), want)
+        for row, pair in enumerate(first):
+            assert pair is None or want[row].tolist() == pair
+
+
 # ------------------------------------------------------------------------------ refusals
 def _router(fmoe, **kw):
     from fmoe_b200.router import FmoeRouter
