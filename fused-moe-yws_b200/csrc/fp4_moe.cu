@@ -273,6 +273,9 @@ extern "C" int fmoe_fp4_forward(const fmoe_fp4_problem* p, const fmoe_fp4_tensor
   for (int i = 0; i < 8; ++i)
     if (!ptrs[i] || reinterpret_cast<uintptr_t>(ptrs[i]) % 16)
       return bad(std::string(names[i]) + " must be non-NULL and 16-byte aligned");
+  for (const float* scale : {t->input_scale, t->intermediate_scale, t->w13_global, t->w2_global})
+    if (reinterpret_cast<uintptr_t>(scale) % 4)
+      return bad("global scales must be aligned to their type");
   if (p->format == FMOE_MXFP4 && (t->input_scale || t->intermediate_scale || t->w13_global ||
                                   t->w2_global))
     return bad("mxfp4 has no global scale");

@@ -367,6 +367,8 @@ int fp4_check_pointers(const fmoe_fp4_matrix* q, const char* name) {
   if (!q->codes || !q->scales) return bad(n + ": codes and scales must not be NULL");
   if (reinterpret_cast<uintptr_t>(q->codes) % 16 || reinterpret_cast<uintptr_t>(q->scales) % 16)
     return bad(n + ": codes and scales must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(q->global_scale) % 4)
+    return bad(n + ": global_scale must be aligned to its type");
   return FMOE_OK;
 }
 
@@ -396,7 +398,8 @@ extern "C" int fmoe_fp4_quantize(const fmoe_fp4_matrix* q, const void* x, int32_
   if (dtype < FMOE_F32 || dtype > FMOE_F16) return bad_dtype("dtype");
   if (q->rows == 0) return FMOE_OK;
   if ((v = fp4_check_pointers(q, "matrix")) != FMOE_OK) return v;
-  if (!x) return bad("x must not be NULL");
+  if (!x || reinterpret_cast<uintptr_t>(x) % (dtype == FMOE_F32 ? 4 : 2))
+    return bad("x must not be NULL and be aligned to its type");
   if (row_stride < 0 || batch_stride < 0) return bad("strides must not be negative");
   Fp4QuantArgs a = args_of(q);
   a.x = x;

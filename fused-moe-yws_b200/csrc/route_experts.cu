@@ -893,6 +893,10 @@ int check_router(const fmoe_router* r) {
   return FMOE_OK;
 }
 
+// Kernels read whole elements: an address between two of them would fault on the device.
+bool off_type(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+size_t logit_bytes(const fmoe_router* r) { return r->logits_dtype == FMOE_F32 ? 4 : 2; }
+
 RouterArgs router_args(const fmoe_router* r, const void* logits) {
   RouterArgs a = {};
   a.logits = logits;
@@ -980,6 +984,9 @@ extern "C" int fmoe_route_experts(const fmoe_router* r, const void* logits, cons
   if (r->num_tokens == 0) return FMOE_OK;
   if (!logits || !out || !out->topk_idx || !out->topk_w)
     return bad("routing pointers must not be NULL");
+  if (off_type(logits, logit_bytes(r)) || off_type(bias, r->bias_dtype == FMOE_F32 ? 4 : 2) ||
+      off_type(out->topk_idx, 4) || off_type(out->topk_w, 4))
+    return bad("routing pointers must be aligned to their type");
   RouterArgs a = router_args(r, logits);
   a.bias = bias;
   a.idx = out->topk_idx;
@@ -995,6 +1002,9 @@ extern "C" int fmoe_route_experts_backward(const fmoe_router* r, const float* gr
   if (r->num_tokens == 0) return FMOE_OK;
   if (!logits || !grad_w || !topk_idx || !grad_logits)
     return bad("routing pointers must not be NULL");
+  if (off_type(logits, logit_bytes(r)) || off_type(grad_logits, logit_bytes(r)) ||
+      off_type(grad_w, 4) || off_type(topk_idx, 4))
+    return bad("routing pointers must be aligned to their type");
   RouterArgs a = router_args(r, logits);
   a.idx = const_cast<int*>(topk_idx);
   a.grad_w = grad_w;

@@ -410,7 +410,7 @@ typedef struct fmoe_fp4_matrix {
 int fmoe_fp4_scale_bytes(const fmoe_fp4_matrix* q, size_t* bytes);
 
 /* Fills q's codes and scales from x: q->batch matrices, row r of matrix b at element
- * b * batch_stride + r * row_stride; dtype is an fmoe_dtype. */
+ * b * batch_stride + r * row_stride; dtype is an fmoe_dtype, x aligned to it. */
 int fmoe_fp4_quantize(const fmoe_fp4_matrix* q, const void* x, int32_t dtype, int64_t row_stride,
                       int64_t batch_stride, void* stream);
 

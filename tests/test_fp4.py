@@ -416,3 +416,19 @@ def test_fp4_rejects_arguments(fmoe):
     short = fmoe.Fp4Tensor(q.codes, q.scales[:, :0], "nvfp4")
     with pytest.raises(ValueError, match="scales"):
         fmoe.dequantize_fp4(short)
+
+
+def test_fp4_rejects_addresses_between_elements(fmoe):
+    """Refused on the host: the kernels would fault on them."""
+    lib = fmoe.load_library()
+    ok, off = _matrix(), _matrix(global_scale=18)
+    for dtype, x in ((0, 18), (1, 17), (2, 33)):
+        assert lib.fmoe_fp4_quantize(ctypes.byref(ok), x, dtype, 64, 0,
+                                     None) == fmoe.FMOE_ERR_VALUE
+        assert b"aligned" in lib.fmoe_last_error()
+    for rc in (lib.fmoe_fp4_quantize(ctypes.byref(off), 16, 0, 64, 0, None),
+               lib.fmoe_fp4_dequantize(ctypes.byref(off), 16, 0, None),
+               lib.fmoe_fp4_matmul(ctypes.byref(off), ctypes.byref(ok), 16, 0, None),
+               lib.fmoe_fp4_matmul(ctypes.byref(ok), ctypes.byref(off), 16, 0, None)):
+        assert rc == fmoe.FMOE_ERR_VALUE
+        assert b"global_scale" in lib.fmoe_last_error()

@@ -507,3 +507,16 @@ def test_forward_fp4_refuses_to_drop_a_gradient(fmoe):
                                "topk_w": (x, torch.autograd.forward_ad.make_dual(w, w))}.items():
             with pytest.raises(ValueError, match=name + ".*tangent"):
                 fmoe.forward_fp4(xx, idx, ww, w13, w2, **kw)
+
+
+def test_fp4_forward_rejects_scales_between_elements(fmoe):
+    from fmoe_b200.fp4 import FmoeFp4Problem, FmoeFp4Tensors
+
+    lib = fmoe.load_library()
+    p = FmoeFp4Problem(4, 256, 128, 8, 2, 0, 1, 1)
+    for f in ("w13_global", "w2_global", "input_scale", "intermediate_scale"):
+        t = FmoeFp4Tensors(*[256] * 12)
+        setattr(t, f, 258)
+        assert lib.fmoe_fp4_forward(ctypes.byref(p), ctypes.byref(t), 256, 1 << 40,
+                                    None) == fmoe.FMOE_ERR_VALUE
+        assert b"global scales" in lib.fmoe_last_error()

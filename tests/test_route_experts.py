@@ -513,3 +513,22 @@ def test_route_experts_refuses_forward_mode_on_the_device(fmoe):
             fmoe.route_experts_backward(torch.autograd.forward_ad.make_dual(w, w), x, idx)
         primal = torch.autograd.forward_ad.unpack_dual(dual).primal
         assert torch.equal(fmoe.route_experts(primal, 2)[0], idx)
+
+
+def test_router_rejects_addresses_between_elements(fmoe):
+    """Refused on the host: the kernels would fault on them."""
+    lib = fmoe.load_library()
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        r = _router(fmoe, logits_dtype=dtype, bias_dtype=min(dtype, 1))
+        p = ctypes.byref(r)
+        for logits, bias, idx, w in ((64 + size // 2, 64, 64, 64), (64, 64 + size // 2, 64, 64),
+                                     (64, None, 66, 64), (64, None, 64, 65)):
+            out = fmoe.FmoeRouteOut(idx, w)
+            assert lib.fmoe_route_experts(p, logits, bias, ctypes.byref(out),
+                                          None) == fmoe.FMOE_ERR_VALUE
+            assert b"aligned" in lib.fmoe_last_error()
+        for grad_w, logits, idx, out in ((66, 64, 64, 64), (64, 64 + size // 2, 64, 64),
+                                         (64, 64, 62, 64), (64, 64, 64, 64 + size // 2)):
+            assert lib.fmoe_route_experts_backward(p, grad_w, logits, idx, out,
+                                                   None) == fmoe.FMOE_ERR_VALUE
+            assert b"aligned" in lib.fmoe_last_error()
